@@ -407,6 +407,102 @@ int qmk_gemm_bf16_nt(const void *W, long long ldw, long long w_batch_stride, int
                      long long a_batch_stride, int rows, int k, int batch, int splits, float *C, long long ldc,
                      long long c_batch_stride, long long c_split_stride, unsigned int *status, cudaStream_t stream);
 
+/* ---- quantized K/V cache -------------------------------------------------
+ * No reference counterpart (its cache is bf16).  K and V rows held in 4 or 8
+ * bits: head_dim is cut into groups of QMK_KV_GROUP values; with a the
+ * largest finite magnitude of a group and L = 7 (4 bits) or 127 (8 bits),
+ *   scale s = bf16(a / L),  code c = clamp(rint(x / s), -L, L)  (0 if s = 0),
+ * and the group stands for s * c.  A NaN is held as 0, an infinity as
+ * +-L * s; either sets QMK_KV_NONFINITE in the status word.
+ * A code is stored with an offset: nibble c + 8 (dimension 2i in the low
+ * half of byte i) or byte c + 128.
+ *
+ * QmkKvCache describes ONE layer: sequence n, K/V head h, position p has its
+ * codes at k_codes + n * code_seq_stride + (h * capacity + p) * head_dim *
+ * bits / 8 (bytes) and its scales at k_scales + n * scale_seq_stride +
+ * (h * capacity + p) * head_dim / 32 (bf16 elements); V alike.  Positions
+ * [0, max_seq_len) may be used; capacity >= max_seq_len is the number of
+ * rows allocated, a multiple of QMK_KV_CAPACITY_STEP (the attention reads
+ * whole tiles; what it reads beyond a row's limit does not count). */
+#define QMK_KV_GROUP 32
+#define QMK_KV_CAPACITY_STEP 128
+
+typedef struct QmkKvCache {
+  void *k_codes;               /* 16-byte aligned, as the other three       */
+  void *v_codes;
+  void *k_scales;              /* bf16                                      */
+  void *v_scales;
+  long long code_seq_stride;   /* bytes, a multiple of 16                   */
+  long long scale_seq_stride;  /* bf16 elements, a multiple of 8            */
+  int num_seqs;
+  int num_kv_heads;
+  int head_dim;                /* 64 or 128                                 */
+  int bits;                    /* 4 or 8                                    */
+  int capacity;
+  int max_seq_len;
+} QmkKvCache;
+
+/* The rows of a call: segment b holds rows row_offsets[b] ..
+ * row_offsets[b + 1] - 1 of the call's row tensors (or row b alone if
+ * row_offsets is NULL, then segments == rows), at positions start[b],
+ * start[b] + 1, ... of sequence seq[b] (or b if seq is NULL).  max_rows: the
+ * most rows that a segment has.  Rows that no segment holds are left as they
+ * are.  A row whose sequence, position or segment start is out of range, or
+ * past max_rows of its segment, sets QMK_KV_BAD_ROW: it is not written, and reads as zeros
+ * (attention: as a row that sees nothing). */
+typedef struct QmkKvRows {
+  int rows;
+  int segments;
+  int max_rows;
+  const int *start;            /* device int32 [segments]                   */
+  const int *row_offsets;      /* device int32 [segments + 1], not decreasing, or NULL */
+  const int *seq;              /* device int32 [segments] or NULL           */
+} QmkKvRows;
+
+/* A [rows, heads, head_dim] tensor: head_dim contiguous, strides in
+ * elements. */
+typedef struct QmkKvTensor {
+  void *data;
+  int dtype;                   /* QMK_BF16, QMK_FP16 or QMK_FP32            */
+  long long row_stride;
+  long long head_stride;
+} QmkKvTensor;
+
+#define QMK_BF16 0
+#define QMK_FP16 1
+#define QMK_FP32 2
+
+#define QMK_KV_BAD_ROW 1u
+#define QMK_KV_NONFINITE 2u
+#define QMK_KV_TIMEOUT 4u
+#define QMK_KV_COPIES_PENDING 8u
+
+/* Quantize rows of k and v into the cache.  A position that a call writes
+ * twice holds either row, value group by value group. */
+int qmk_kv_write(const QmkKvCache *cache, const QmkKvRows *rows, const QmkKvTensor *k, const QmkKvTensor *v,
+                 unsigned int *status, cudaStream_t stream);
+
+/* Read rows back: the values they stand for, rounded to k's and v's type. */
+int qmk_kv_read(const QmkKvCache *cache, const QmkKvRows *rows, const QmkKvTensor *k, const QmkKvTensor *v,
+                unsigned int *status, cudaStream_t stream);
+
+/* Causal attention over the cache: q [rows, num_q_heads, head_dim] with
+ * num_q_heads a multiple (1 .. QMK_KV_MAX_RATIO) of num_kv_heads, q head j
+ * reading K/V head j / (num_q_heads / num_kv_heads).  The row at position p
+ * attends to positions 0 .. p of its sequence, which must have been written:
+ *   out = sum_j softmax_j(scale * q . k_j) v_j.
+ * out has q's type.  Scores, sums and the softmax are fp32.  A wait that
+ * exceeds 1 s sets QMK_KV_TIMEOUT (the outputs are then invalid), and
+ * QMK_KV_COPIES_PENDING if copies were still in flight a second later.
+ * The workspace (qmk_kv_attend_workspace_bytes, 256-byte aligned) needs no
+ * initialization; calls that overlap in time need one each. */
+#define QMK_KV_MAX_RATIO 16
+
+size_t qmk_kv_attend_workspace_bytes(const QmkKvCache *cache, const QmkKvRows *rows, int num_q_heads, int dtype);
+int qmk_kv_attend(const QmkKvCache *cache, const QmkKvRows *rows, const QmkKvTensor *q, int num_q_heads,
+                  const QmkKvTensor *out, float scale, void *workspace, size_t workspace_bytes,
+                  unsigned int *status, cudaStream_t stream);
+
 /* Library version string. */
 const char *qmk_version(void);
 

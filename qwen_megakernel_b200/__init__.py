@@ -10,6 +10,7 @@ The native libraries are loaded on first use (``Decoder(...)`` or
 
 from .model import Decoder, DecodeError, generate, load_weights, random_weights  # noqa: F401
 from .batch import BatchDecoder, BatchError, BatchForward  # noqa: F401
+from .kv_cache import KVCacheError, KVRows, QuantKVCache  # noqa: F401
 from .weights import rope_tables  # noqa: F401
 from ._native import ops, cdll  # noqa: F401
 
@@ -22,6 +23,9 @@ __all__ = [
     "BatchDecoder",
     "BatchError",
     "BatchForward",
+    "KVCacheError",
+    "KVRows",
+    "QuantKVCache",
     "generate",
     "ops",
     "cdll",

@@ -18,6 +18,8 @@
 //   default_status()     -> qmk_read_default_status (after a synchronize)
 //   num_ctas()           -> qmk_num_ctas(current device)
 //   trace_words()        -> qmk_trace_words
+//   kv_write / kv_read / kv_attend -> qmk_kv_write / qmk_kv_read / qmk_kv_attend:
+//                           the quantized K/V cache
 #include <Python.h>
 
 #include <c10/cuda/CUDAGuard.h>
@@ -29,6 +31,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
+#include <string>
 
 #include "qwen_megakernel.h"
 
@@ -478,6 +481,160 @@ int64_t batch_workspace_bytes(int64_t num_rows, int64_t num_out) {
   return (int64_t)n;
 }
 
+// ---- quantized K/V cache ----------------------------------------------------
+// Cache tensors: codes uint8 [num_seqs, layers, heads, capacity, head_dim * bits / 8]
+// and scales bf16 [num_seqs, layers, heads, capacity, head_dim / 32], contiguous.
+struct KvCall {
+  QmkKvCache cache;
+  QmkKvRows rows;
+  unsigned *status = nullptr;
+};
+
+KvCall kv_call(const torch::Tensor &k_codes, const torch::Tensor &v_codes, const torch::Tensor &k_scales,
+               const torch::Tensor &v_scales, int64_t bits, int64_t max_seq_len, int64_t layer, int64_t rows,
+               const torch::Tensor &start, const std::optional<torch::Tensor> &row_offsets,
+               const std::optional<torch::Tensor> &seq, int64_t max_rows, const std::optional<torch::Tensor> &status) {
+  check_dtype(k_codes, torch::kUInt8, "k_codes", "uint8");
+  check_dtype(v_codes, torch::kUInt8, "v_codes", "uint8");
+  check_dtype(k_scales, torch::kBFloat16, "k_scales", "bfloat16");
+  check_dtype(v_scales, torch::kBFloat16, "v_scales", "bfloat16");
+  for (const auto *t : {&v_codes, &k_scales, &v_scales}) check_same_device(*t, k_codes, "cache tensor");
+  QMK_CHECK(bits == 4 || bits == 8, "bits must be 4 or 8, got %lld", (ll)bits);
+  QMK_CHECK(k_codes.dim() == 5 && k_scales.dim() == 5,
+            "codes must be [num_seqs, layers, heads, capacity, head_dim * bits / 8] and scales [num_seqs, layers, "
+            "heads, capacity, head_dim / %d]",
+            QMK_KV_GROUP);
+  QMK_CHECK(v_codes.sizes() == k_codes.sizes() && v_scales.sizes() == k_scales.sizes(), "v must match k in shape");
+  const int64_t head_dim = k_codes.size(4) * 8 / bits;
+  for (int i = 0; i < 4; ++i)
+    QMK_CHECK(k_scales.size(i) == k_codes.size(i), "scales must match codes in dimension %d", i);
+  QMK_CHECK(k_scales.size(4) * QMK_KV_GROUP == head_dim, "scales must hold one value for %d", QMK_KV_GROUP);
+  QMK_CHECK(layer >= 0 && layer < k_codes.size(1), "layer %lld outside [0, %lld)", (ll)layer, (ll)k_codes.size(1));
+  QMK_CHECK(max_seq_len >= 1 && max_seq_len <= k_codes.size(3), "max_seq_len %lld outside [1, capacity %lld]",
+            (ll)max_seq_len, (ll)k_codes.size(3));
+  QMK_CHECK(k_codes.size(0) < INT32_MAX && k_codes.size(3) < INT32_MAX, "cache dimensions must fit 32 bits");
+  check_dtype(start, torch::kInt32, "start", "int32");
+  check_same_device(start, k_codes, "start");
+  QMK_CHECK(start.dim() == 1, "start must be one-dimensional");
+  QMK_CHECK(rows < INT32_MAX && start.numel() < INT32_MAX, "too many rows");
+  const int64_t segments = start.numel();
+  KvCall c;
+  auto at = [&](const torch::Tensor &t) {
+    return static_cast<uint8_t *>(t.data_ptr()) + layer * t.stride(1) * (int64_t)t.element_size();
+  };
+  c.cache = QmkKvCache{at(k_codes),          at(v_codes),
+                       at(k_scales),         at(v_scales),
+                       k_codes.stride(0),    k_scales.stride(0),
+                       (int)k_codes.size(0), (int)k_codes.size(2),
+                       (int)head_dim,        (int)bits,
+                       (int)k_codes.size(3), (int)max_seq_len};
+  QMK_CHECK(max_rows >= 0 && max_rows <= max_seq_len, "max_rows %lld outside [0, max_seq_len %lld]", (ll)max_rows,
+            (ll)max_seq_len);
+  c.rows = QmkKvRows{(int)rows, (int)segments, (int)max_rows, static_cast<const int *>(start.data_ptr()), nullptr,
+                     nullptr};
+  if (row_offsets.has_value()) {
+    check_dtype(*row_offsets, torch::kInt32, "row_offsets", "int32");
+    check_same_device(*row_offsets, k_codes, "row_offsets");
+    QMK_CHECK(row_offsets->numel() == segments + 1, "row_offsets must have %lld elements", (ll)(segments + 1));
+    c.rows.row_offsets = static_cast<const int *>(row_offsets->data_ptr());
+  } else {
+    QMK_CHECK(segments == rows, "%lld rows for %lld segments need row_offsets", (ll)rows, (ll)segments);
+  }
+  if (seq.has_value()) {
+    check_dtype(*seq, torch::kInt32, "seq", "int32");
+    check_same_device(*seq, k_codes, "seq");
+    QMK_CHECK(seq->numel() == segments, "seq must have %lld elements", (ll)segments);
+    c.rows.seq = static_cast<const int *>(seq->data_ptr());
+  }
+  if (status.has_value()) {
+    check_dtype(*status, torch::kInt32, "status", "int32");
+    check_same_device(*status, k_codes, "status");
+    QMK_CHECK(status->numel() >= 1, "status must hold an element");
+    c.status = reinterpret_cast<unsigned *>(status->data_ptr());
+  }
+  return c;
+}
+
+// A [rows, heads, head_dim] tensor of floating-point values, head_dim contiguous.
+QmkKvTensor kv_tensor(const torch::Tensor &t, const torch::Tensor &like, const char *name, int64_t heads,
+                      int64_t head_dim) {
+  QMK_CHECK(t.is_cuda(), "%s must be a CUDA tensor", name);
+  QMK_CHECK(t.device() == like.device(), "%s is on cuda:%d but the cache is on cuda:%d", name,
+            (int)t.device().index(), (int)like.device().index());
+  QMK_CHECK(t.dim() == 3 && t.size(2) == head_dim && (heads < 0 || t.size(1) == heads),
+            "%s must be [rows, heads%s%lld, head_dim=%lld]", name, heads < 0 ? ">=" : "=",
+            (ll)(heads < 0 ? 1 : heads), (ll)head_dim);
+  QMK_CHECK(t.stride(2) == 1 || t.numel() == 0, "%s must be contiguous along head_dim", name);
+  QmkKvTensor out;
+  out.data = t.data_ptr();
+  switch (t.scalar_type()) {
+    case torch::kBFloat16: out.dtype = QMK_BF16; break;
+    case torch::kHalf: out.dtype = QMK_FP16; break;
+    case torch::kFloat: out.dtype = QMK_FP32; break;
+    default: fail("%s must be bfloat16, float16 or float32", name);
+  }
+  out.row_stride = t.stride(0);
+  out.head_stride = t.stride(1);
+  return out;
+}
+
+// A tensor that a call writes must not hold an element twice (an expanded one does).
+void check_writable(const torch::Tensor &t, const char *name) {
+  QMK_CHECK((t.size(0) <= 1 || t.stride(0) != 0) && (t.size(1) <= 1 || t.stride(1) != 0),
+            "%s must not be an expanded tensor", name);
+}
+
+void kv_write(torch::Tensor k_codes, torch::Tensor v_codes, torch::Tensor k_scales, torch::Tensor v_scales,
+              int64_t bits, int64_t max_seq_len, int64_t layer, torch::Tensor k, torch::Tensor v, torch::Tensor start,
+              std::optional<torch::Tensor> row_offsets, std::optional<torch::Tensor> seq, int64_t max_rows,
+              std::optional<torch::Tensor> status) {
+  const KvCall c = kv_call(k_codes, v_codes, k_scales, v_scales, bits, max_seq_len, layer, k.dim() ? k.size(0) : 0,
+                           start, row_offsets, seq, max_rows, status);
+  const QmkKvTensor kt = kv_tensor(k, k_codes, "k", c.cache.num_kv_heads, c.cache.head_dim);
+  const QmkKvTensor vt = kv_tensor(v, k_codes, "v", c.cache.num_kv_heads, c.cache.head_dim);
+  QMK_CHECK(v.size(0) == k.size(0) && v.scalar_type() == k.scalar_type(), "v must match k in rows and type");
+  if (k.size(0) == 0) return;
+  c10::cuda::CUDAGuard guard(k_codes.device());
+  raise_if_error(qmk_kv_write(&c.cache, &c.rows, &kt, &vt, c.status, c10::cuda::getCurrentCUDAStream().stream()));
+}
+
+void kv_read(torch::Tensor k_codes, torch::Tensor v_codes, torch::Tensor k_scales, torch::Tensor v_scales,
+             int64_t bits, int64_t max_seq_len, int64_t layer, torch::Tensor k, torch::Tensor v, torch::Tensor start,
+             std::optional<torch::Tensor> row_offsets, std::optional<torch::Tensor> seq, int64_t max_rows,
+             std::optional<torch::Tensor> status) {
+  const KvCall c = kv_call(k_codes, v_codes, k_scales, v_scales, bits, max_seq_len, layer, k.dim() ? k.size(0) : 0,
+                           start, row_offsets, seq, max_rows, status);
+  const QmkKvTensor kt = kv_tensor(k, k_codes, "k", c.cache.num_kv_heads, c.cache.head_dim);
+  const QmkKvTensor vt = kv_tensor(v, k_codes, "v", c.cache.num_kv_heads, c.cache.head_dim);
+  check_writable(k, "k");
+  check_writable(v, "v");
+  QMK_CHECK(v.size(0) == k.size(0) && v.scalar_type() == k.scalar_type(), "v must match k in rows and type");
+  if (k.size(0) == 0) return;
+  c10::cuda::CUDAGuard guard(k_codes.device());
+  raise_if_error(qmk_kv_read(&c.cache, &c.rows, &kt, &vt, c.status, c10::cuda::getCurrentCUDAStream().stream()));
+}
+
+// The workspace comes from the caching allocator on the current stream, so
+// calls on several streams and captured graphs never share one.
+void kv_attend(torch::Tensor k_codes, torch::Tensor v_codes, torch::Tensor k_scales, torch::Tensor v_scales,
+               int64_t bits, int64_t max_seq_len, int64_t layer, torch::Tensor q, torch::Tensor out,
+               torch::Tensor start, std::optional<torch::Tensor> row_offsets, std::optional<torch::Tensor> seq,
+               int64_t max_rows, double scale, std::optional<torch::Tensor> status) {
+  const KvCall c = kv_call(k_codes, v_codes, k_scales, v_scales, bits, max_seq_len, layer, q.dim() ? q.size(0) : 0,
+                           start, row_offsets, seq, max_rows, status);
+  const QmkKvTensor qt = kv_tensor(q, k_codes, "q", -1, c.cache.head_dim);
+  const QmkKvTensor ot = kv_tensor(out, k_codes, "out", q.size(1), c.cache.head_dim);
+  check_writable(out, "out");
+  QMK_CHECK(out.size(0) == q.size(0) && out.scalar_type() == q.scalar_type(), "out must match q in rows and type");
+  if (q.size(0) == 0) return;
+  c10::cuda::CUDAGuard guard(k_codes.device());
+  const size_t need = qmk_kv_attend_workspace_bytes(&c.cache, &c.rows, (int)q.size(1), qt.dtype);
+  if (need == 0) raise_if_error(qmk_get_last_error());
+  torch::Tensor ws = torch::empty({(int64_t)need}, k_codes.options());
+  raise_if_error(qmk_kv_attend(&c.cache, &c.rows, &qt, (int)q.size(1), &ot, (float)scale, ws.data_ptr(), need,
+                               c.status, c10::cuda::getCurrentCUDAStream().stream()));
+}
+
 int64_t workspace_bytes() { return (int64_t)qmk_workspace_bytes(); }
 
 void workspace_init(torch::Tensor workspace) {
@@ -561,6 +718,18 @@ TORCH_LIBRARY(qwen_megakernel_C, ops) {
       "Tensor? logits, Tensor? status, int causal_run=0) -> ()");
   ops.impl("batch_forward", torch::kCUDA, &batch_forward);
   ops.def("batch_workspace_bytes(int num_rows, int num_out) -> int", &batch_workspace_bytes);
+
+  const char *kv_rows_args =
+      "Tensor start, Tensor? row_offsets, Tensor? seq, int max_rows";
+  const std::string kv_cache_args =
+      "Tensor k_codes, Tensor v_codes, Tensor k_scales, Tensor v_scales, int bits, int max_seq_len, int layer, ";
+  ops.def(("kv_write(" + kv_cache_args + "Tensor k, Tensor v, " + kv_rows_args + ", Tensor? status) -> ()").c_str());
+  ops.impl("kv_write", torch::kCUDA, &kv_write);
+  ops.def(("kv_read(" + kv_cache_args + "Tensor k, Tensor v, " + kv_rows_args + ", Tensor? status) -> ()").c_str());
+  ops.impl("kv_read", torch::kCUDA, &kv_read);
+  ops.def(("kv_attend(" + kv_cache_args + "Tensor q, Tensor out, " + kv_rows_args +
+           ", float scale, Tensor? status) -> ()").c_str());
+  ops.impl("kv_attend", torch::kCUDA, &kv_attend);
 
   ops.def("workspace_bytes() -> int", &workspace_bytes);
   ops.def("workspace_init(Tensor workspace) -> ()");
