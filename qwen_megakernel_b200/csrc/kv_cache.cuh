@@ -30,7 +30,7 @@ __device__ __forceinline__ void segment_rows(const Rows &R, int b, int &r0, int 
     return;
   }
   r0 = min(max(R.row_offsets[b], 0), R.rows);
-  n = max(min(R.row_offsets[b + 1], R.rows) - r0, 0);
+  n = max(min(max(R.row_offsets[b + 1], 0), R.rows) - r0, 0);
 }
 
 __device__ __forceinline__ int segment_seq(const Rows &R, int b) { return R.seq ? R.seq[b] : b; }
@@ -47,7 +47,7 @@ __device__ __forceinline__ int locate_row(const Rows &R, int r, int &seq, int &p
       else hi = mid;
     }
     b = lo;
-    i = r - R.row_offsets[b];
+    i = r - max(R.row_offsets[b], 0);
     if (i < 0 || r >= R.row_offsets[b + 1]) return 0;
     if (i >= R.max_rows) return -1;
   }

@@ -2,23 +2,24 @@
 
 Tolerances.  Held values are compared exactly: codes and scales are fixed by
 the format.  For the attention, with e_t = torch.finfo(t).eps / 2 the half
-step of q's type, A = sum_j p_j |v_j| / sum_j p_j and S = scale * max_j sum_d
-|q_d| s_jd C, where s is a value's scale and C the range of an offset code (16
-or 256), an output may be off by
+step of q's type, A = sum_j p_j |v_j| / sum_j p_j and K = scale * max_j sum_d
+|q_d k_jd|, an output may be off by
 
-    e_t max(|out|, tiny_t) + (P + 2 * 2^-18 S + 2^-18) A
+    e_t max(|out|, tiny_t) + (P + 2 * 2^-18 K + 2^-18) A + 2^-39 n max |v|
 
 * the first term is the rounding to q's type; below the smallest normal
   number tiny_t its steps stay those at tiny_t, 2 e_t tiny_t (fp16: 2^-24);
-* P: the probabilities (and 8-bit values, the queries) enter the tensor cores
-  as one fp16 each for 16-bit types, three roundings of 2^-11 at most on a
-  product p_j v_j or q_d k_jd; as fp16 pairs for fp32, 2^-20;
-* 2^-18 S bounds the fp32 error of a score, up to 2^6 additions of terms that
-  carry the codes' offset, each off by 2^-24 of the sum of magnitudes; an
-  error of a score is a relative error of its p and of the sum of p, so it
-  counts twice.  For 16-bit types the rounding of 8-bit keys to fp16 adds up
-  to 2^-11 of scale * max_j sum_d |q_d k_jd|, also twice;
-* 2^-18: sums of p and p v in fp32, exp2 and the final division.
+* P: for 16-bit types the probabilities enter the tensor cores as one fp16
+  each, and so may the 8-bit values and keys: three roundings of 2^-11 at most
+  on a product p_j v_j; for fp32 as fp16 pairs, 2^-20;
+* 2^-18 K bounds the fp32 error of a score, up to 2^6 additions each off by
+  2^-24 of the sum of magnitudes; an error of a score is a relative error of
+  its p and of the sum of p, so it counts twice.  For 16-bit types the rounding
+  of 8-bit keys to fp16 adds up to 2^-11 K, also twice;
+* 2^-18: sums of p and p v in fp32, exp2 and the final division;
+* a product p_j s_j, taken relative to the largest p and s so that it lies
+  below 2^15, is never held finer than fp16's last half step 2^-25: 2^-40 of
+  the largest, and s_j times a code is at most max |v|; n terms, doubled.
 """
 
 import math
@@ -34,14 +35,14 @@ TYPES = [torch.bfloat16, torch.float16, torch.float32]
 
 
 def held(x, bits):
-    """The values that rows x stand for once held, and their scales, in 64 bits."""
+    """The values that rows x stand for once held, in 64 bits."""
     top = 7 if bits == 4 else 127
     g = x.double().unflatten(-1, (-1, 32))
     fin = torch.where(g.isfinite(), g, 0.0)
     s = (fin.abs().amax(-1, keepdim=True) / top).bfloat16().double()
     c = (g / torch.where(s > 0, s, 1.0)).round().clamp(-top, top)
     c = torch.where((s > 0) & ~g.isnan(), c, 0.0)
-    return (c * s).flatten(-2), s.expand_as(g).flatten(-2)
+    return (c * s).flatten(-2)
 
 
 def attention(q, k, v, limits, scale):
@@ -56,21 +57,17 @@ def attention(q, k, v, limits, scale):
     return torch.einsum("hnm,mhd->nhd", p, v), torch.einsum("hnm,mhd->nhd", p, v.abs())
 
 
-def check_attend(got, q, k, v, ks, limits, bits, scale):
-    """got against the formulas; ks: scales of k."""
+def check_attend(got, q, k, v, limits, bits, scale):
+    """got against the formulas."""
     ref, A = attention(q, k, v, limits, scale)
-    ratio = q.shape[1] // k.shape[1]
-    live = max(limits)
-    qa = q.double().abs()
-    C = 16 if bits == 4 else 256
-    S = scale * torch.einsum("nhd,mhd->nhm", qa, ks[:live].repeat_interleave(ratio, 1)).amax(-1, keepdim=True) * C
-    K = scale * torch.einsum("nhd,mhd->nhm", qa, k[:live].abs().repeat_interleave(ratio, 1)).amax(-1, keepdim=True)
+    seen = k[:max(limits)].abs().repeat_interleave(q.shape[1] // k.shape[1], 1)
+    K = scale * torch.einsum("nhd,mhd->nhm", q.double().abs(), seen).amax(-1, keepdim=True)
     low = q.dtype != torch.float32
     P = 3 * 2.0**-11 if low else 2.0**-20
     if low and bits == 8:
         P = P + 2 * 2.0**-11 * K
     e = torch.finfo(q.dtype).eps / 2
-    tol = e * ref.abs().clamp(min=torch.finfo(q.dtype).tiny) + (P + 2 * 2.0**-18 * S + 2.0**-18) * A + 1e-30
+    tol = e * ref.abs().clamp(min=torch.finfo(q.dtype).tiny) + (P + 2 * 2.0**-18 * K + 2.0**-18) * A + 2.0**-39 * max(limits) * v.abs().max()
     bad = (got.double() - ref).abs() > tol
     assert not bad.any(), (f"{int(bad.sum())} of {bad.numel()} off; worst "
                            f"{((got.double() - ref).abs() / tol).max().item():.2f} of the tolerance")
@@ -99,9 +96,9 @@ class Filled:
         r = 0
         for seq, start, n in segs:
             if n:
-                k, ks = held(self.k[seq], self.bits)
-                v, _ = held(self.v[seq], self.bits)
-                check_attend(got[r:r + n], q[r:r + n], k, v, ks, [start + i + 1 for i in range(n)], self.bits, scale)
+                k = held(self.k[seq], self.bits)
+                v = held(self.v[seq], self.bits)
+                check_attend(got[r:r + n], q[r:r + n], k, v, [start + i + 1 for i in range(n)], self.bits, scale)
             r += n
 
 
@@ -140,7 +137,7 @@ def test_write_read_exact(dtype, bits, d):
     for t in TYPES:
         kr, vr = cache.read(rows, layer=1, dtype=t)
         # exact values have at most 15 bits: one rounding, to t
-        assert torch.equal(kr, held(k, bits)[0].float().to(t)) and torch.equal(vr, held(v, bits)[0].float().to(t))
+        assert torch.equal(kr, held(k, bits).float().to(t)) and torch.equal(vr, held(v, bits).float().to(t))
     # (some of the spread values lie past fp16's range: infinities, reported)
     if torch.isfinite(k).all() and torch.isfinite(v).all():
         cache.check_status()
@@ -166,7 +163,7 @@ def test_write_nonfinite():
     with pytest.raises(KVCacheError, match="NaN or infinity"):
         cache.check_status()
     k, v = cache.read(rows, dtype=torch.float32)
-    assert torch.equal(k, held(x, 4)[0].float()) and not v.any() and torch.isfinite(k).all()
+    assert torch.equal(k, held(x, 4).float()) and not v.any() and torch.isfinite(k).all()
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
@@ -186,7 +183,7 @@ def test_strides_and_alignment(dtype):
         out = torch.full((n, hk * d * 2 + 3), 7.0, dtype=dtype, device="cuda")
         kr, vr = out[:, off:off + hk * d].unflatten(1, (hk, d)), out[:, -hk * d:].unflatten(1, (hk, d))
         cache.read(rows, out=(kr, vr))
-        assert torch.equal(kr, held(k, 4)[0].float().to(dtype)) and torch.equal(vr, held(v, 4)[0].float().to(dtype))
+        assert torch.equal(kr, held(k, 4).float().to(dtype)) and torch.equal(vr, held(v, 4).float().to(dtype))
         rest = torch.ones(out.shape[1], dtype=torch.bool)
         rest[off:off + hk * d] = False
         rest[-hk * d:] = False
@@ -359,14 +356,14 @@ def test_offsets_past_32_bits():
     c.write(k, v, KVRows([0], [n], [seqs - 1]))
     rows = KVRows([n - 5], [5], [seqs - 1])
     kr, vr = c.read(rows, dtype=torch.float32)
-    assert torch.equal(kr, held(k[-5:], 8)[0].float()) and torch.equal(vr, held(v[-5:], 8)[0].float())
+    assert torch.equal(kr, held(k[-5:], 8).float()) and torch.equal(vr, held(v[-5:], 8).float())
     assert not c.k_codes[:seqs - 1, :, :, -8:].any()
     q = torch.randn(5, 8, 128, generator=g, device="cuda", dtype=torch.bfloat16)
     got = c.attend(q, rows)
     for h in (0, 7):
-        kh, ks = held(k[:, h:h + 1], 8)
-        check_attend(got[:, h:h + 1], q[:, h:h + 1], kh, held(v[:, h:h + 1], 8)[0], ks, [n - 4 + i for i in range(5)],
-                     8, 1 / math.sqrt(128))
+        kh, vh = held(k[:, h:h + 1], 8), held(v[:, h:h + 1], 8)
+        check_attend(got[:, h:h + 1], q[:, h:h + 1], kh, vh, [n - 4 + i for i in range(5)], 8,
+                     1 / math.sqrt(128))
 
 
 def test_repeatable_and_independent_of_neighbours():
@@ -417,8 +414,8 @@ def test_graph_replay_with_moving_positions():
         kb.copy_(k[t]), vb.copy_(v[t]), qb.copy_(q[t])
         graphs[t % 2].replay()
         for s in range(2):
-            kh, ks = held(k[:t + 1, s], 4)
-            check_attend(out[s:s + 1], q[t, s:s + 1], kh, held(v[:t + 1, s], 4)[0], ks, [t + 1], 4, 1 / math.sqrt(d))
+            kh, vh = held(k[:t + 1, s], 4), held(v[:t + 1, s], 4)
+            check_attend(out[s:s + 1], q[t, s:s + 1], kh, vh, [t + 1], 4, 1 / math.sqrt(d))
     c.check_status()
 
 
@@ -442,9 +439,9 @@ def test_prompt_then_steps_together():
         for s, n in enumerate(counts):
             ks[s].append(k[r:r + n])
             vs[s].append(v[r:r + n])
-            kh, sc = held(torch.cat(ks[s]), 8)
-            check_attend(out[r:r + n], q[r:r + n], kh, held(torch.cat(vs[s]), 8)[0], sc,
-                         [starts[s] + i + 1 for i in range(n)], 8, 1 / math.sqrt(d))
+            kh, vh = held(torch.cat(ks[s]), 8), held(torch.cat(vs[s]), 8)
+            check_attend(out[r:r + n], q[r:r + n], kh, vh, [starts[s] + i + 1 for i in range(n)], 8,
+                         1 / math.sqrt(d))
             r += n
 
     feed(lens, [0, 0, 0])
