@@ -15,8 +15,8 @@
 //
 // Precision: q is scaled per row by a power of two into fp16's range; bf16
 // and fp16 queries lose nothing by it (elements 2^-24 below the row's
-// largest aside).  p s is scaled per tile by the power of two e of the
-// tile's largest scale, with the running maximum taken of score + e, and
+// largest aside).  p s keeps to fp16's range by taking the running maximum
+// of score + e, 2^e the power of two of a tile's largest scale; it is
 // rounded to fp16 (2^-11 of a term); fp32 queries are split into an fp16
 // pair hi + lo on two columns of the same product, as is p s (2^-22).
 // Scores, maxima, sums and outputs are fp32.
@@ -40,7 +40,7 @@ constexpr unsigned long long kWaitNs = 1000000000ull;  // bound on one copy wait
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttendArgs {
-  CUtensorMap k_map, v_map;  // codes: dims {row bytes, capacity, heads, sequences}
+  CUtensorMap k_map, v_map;  // codes: dims {128 bytes, 128-byte lines, heads, sequences}
   const __nv_bfloat16 *k_scales, *v_scales;
   long long scale_seq_stride;
   int capacity, heads, ratio;
@@ -50,18 +50,19 @@ struct AttendArgs {
   long long q_row, q_head, o_row, o_head;
   bool q_aligned;
   float scale_log2;  // softmax scale * log2(e)
-  int *desc;         // workspace: per CTA 2 part descriptors of kDescWords
-  float *parts;      // workspace: per CTA 2 x slots x (D + 2)
+  int *desc;         // workspace: per worker a descriptor of kDescWords
+  float *parts;      // workspace: per worker 2 x slots x (D + 4)
   unsigned *status;
 };
 
 // ------------------------------------------------------------- work division
-// The query rows of one segment and K/V head are cut into blocks of RB rows
-// by HB of the K/V head's q heads; a block and its positions [0, len), in
+// The query rows of one segment and K/V head are cut into blocks of rb rows
+// by hb of the K/V head's q heads; a block and its positions [0, len), in
 // tiles, are an item.  All items' tiles in order (segment, K/V head, head
-// block, row block) form one list that is dealt to the CTAs in equal
-// contiguous ranges, so ragged lengths and few items both load every SM; an
-// item cut by a range border leaves parts that merge_kernel joins.
+// block, row block) form one list that is dealt to the workers (warps) in
+// equal contiguous ranges, so ragged lengths, few items and many all load
+// every SM alike; an item cut by a range border leaves parts that
+// merge_kernel joins, in order.
 struct Segment {
   int r0, n;      // rows
   int ok_rows;    // the first ok_rows of them are in range
@@ -125,7 +126,7 @@ constexpr int kDescWords = 8;
 // ------------------------------------------------------------- instructions
 __device__ __forceinline__ void mma_f16(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
                                         unsigned b1, float c0, float c1, float c2, float c3) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%10, %11, %12, %13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
@@ -149,7 +150,12 @@ __device__ __forceinline__ void ldmatrix4_trans(unsigned (&r)[4], uint32_t addr)
 }
 __device__ __forceinline__ unsigned transpose8(unsigned x) {
   unsigned y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ unsigned max_u16x2(unsigned a, unsigned b) {
+  unsigned y;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
   return y;
 }
 __device__ __forceinline__ float fast_exp2(float x) {
@@ -171,19 +177,34 @@ __device__ __forceinline__ unsigned hfma2(unsigned x, unsigned m, unsigned c) {
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(y) : "r"(x), "r"(m), "r"(c));
   return y;
 }
-// The fp16 values u - 8 of nibbles (0, 4), (1, 5), (2, 6), (3, 7) of w.
-__device__ __forceinline__ void decode4(unsigned w, unsigned (&h)[4]) {
-  const unsigned v = w >> 8;
-  h[0] = hadd2((w & 0x000f000fu) | 0x64006400u, 0xe408e408u);               // - 1032
-  h[1] = hfma2((w & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd480d480u);  // / 16 - 72
-  h[2] = hadd2((v & 0x000f000fu) | 0x64006400u, 0xe408e408u);
-  h[3] = hfma2((v & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd480d480u);
-}
-// The fp16 values u - 128 of bytes (0, 2) and (1, 3) of w.
-__device__ __forceinline__ void decode8(unsigned w, unsigned (&h)[2]) {
-  h[0] = hadd2(__byte_perm(w, 0x64646464u, 0x4240), 0xe480e480u);  // - 1152
-  h[1] = hadd2(__byte_perm(w, 0x64646464u, 0x4341), 0xe480e480u);
-}
+// Constants of the decoding, kept in registers: an instruction takes one
+// immediate operand, and these are second ones.
+struct Decode {
+  unsigned exp, off;
+  __device__ __forceinline__ explicit Decode(int bits) {
+    asm volatile("mov.b32 %0, %1;" : "=r"(exp) : "r"(bits == 4 ? 0x64006400u : 0x64646464u));
+    asm volatile("mov.b32 %0, %1;" : "=r"(off) : "r"(0xd480d480u));  // -72
+  }
+  template <unsigned MASK>
+  __device__ __forceinline__ unsigned take(unsigned w) const {  // (w & MASK) | exp
+    unsigned y;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(y) : "r"(w), "n"(MASK), "r"(exp));
+    return y;
+  }
+  // The fp16 values u - 8 of nibbles (0, 4), (1, 5), (2, 6), (3, 7) of w.
+  __device__ __forceinline__ void nibbles(unsigned w, unsigned (&h)[4]) const {
+    const unsigned v = w >> 8;
+    h[0] = hadd2(take<0x000f000fu>(w), 0xe408e408u);        // 1024 + u - 1032
+    h[1] = hfma2(take<0x00f000f0u>(w), 0x2c002c00u, off);  // (1024 + 16 u) / 16 - 72
+    h[2] = hadd2(take<0x000f000fu>(v), 0xe408e408u);
+    h[3] = hfma2(take<0x00f000f0u>(v), 0x2c002c00u, off);
+  }
+  // The fp16 values u - 128 of bytes (0, 2) and (1, 3) of w.
+  __device__ __forceinline__ void bytes(unsigned w, unsigned (&h)[2]) const {
+    h[0] = hadd2(__byte_perm(w, exp, 0x4240), 0xe480e480u);  // 1024 + u - 1152
+    h[1] = hadd2(__byte_perm(w, exp, 0x4341), 0xe480e480u);
+  }
+};
 __device__ __forceinline__ float f16_round(float x) { return __half2float(__float2half_rn(x)); }
 
 __device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, int x, int y, int z, int w,
@@ -208,38 +229,37 @@ __device__ __forceinline__ bool wait_copy(uint64_t *bar, unsigned parity) {
 }
 
 // ------------------------------------------------------------------- kernel
-// A CTA is 4 warps that share an item; warp w takes its tiles w, w + 4, ...
-// of 32 positions through a ring of its own (codes by TMA with the swizzle
-// that makes 8 rows of a 16-byte column free of bank conflicts for ldmatrix,
-// scales by 1-D bulk copies), with its own running maximum, sum and output:
-// no barrier between warps inside an item.  Score product: M = 16 positions,
-// N = 8 columns (query rows x heads; hi and lo apart for fp32), K = 16
-// dimensions.  Output product: M = 16 dimensions, N = the same columns,
-// K = 16 positions, the code words transposed by ldmatrix.
-constexpr int kWarps = 4;
-constexpr int kTile = 32;
-constexpr float kShift = 14.f;  // p is held 2^14 times too large: p s < 2^15 fits fp16, and its small values do too
+// Every warp is a worker of its own: it walks its range of the tile list with
+// a private ring of tiles (codes by TMA, as 128-byte lines under the 128-byte
+// swizzle, which leaves 8 positions of a 16-byte column free of bank conflicts
+// for ldmatrix; scales by 1-D bulk copies) and a running maximum, sum and
+// output in registers; warps never wait for one another.  Score product: M =
+// 16 positions, N = 8 columns (query rows x heads; hi and lo apart for fp32),
+// K = 16 dimensions.  Output product: M = 16 dimensions, N = the same columns,
+// K = 16 positions, the code words transposed by ldmatrix, p transposed in
+// registers.
+// p is held 2^14 times too large: p s < 2^15 fits fp16, and so do its small values
+constexpr float kShift = 14.f;
 
 template <typename T, int BITS, int D, int NT>
 struct Shape {
   static constexpr bool kSplit = sizeof(T) == 4;
-  static constexpr int kPerTile = kSplit ? 4 : 8;
-  static constexpr int kSlots = NT * kPerTile;  // (row, head) pairs of an item
+  static constexpr int kSlots = NT * (kSplit ? 4 : 8);  // (row, head) pairs of an item
   static constexpr int kGroups = D / kGroup;
   static constexpr int kRowBytes = D * BITS / 8;
   static constexpr int kChunks = kRowBytes / 16;
+  static constexpr int kTile = kRowBytes == 128 ? 32 : 64;  // positions
   static constexpr int kCodeBytes = kTile * kRowBytes;
   static constexpr int kScaleBytes = kTile * kGroups * 2;
   static constexpr int kTxBytes = 2 * (kCodeBytes + kScaleBytes);
   static constexpr int kStageBytes = (kTxBytes + 1023) / 1024 * 1024;
-  static constexpr int kCtas = NT == 1 && kRowBytes < 128 ? 3 : 2;  // per SM
-  static constexpr int kStages = std::min(6, (224 * 1024 / kCtas - 2048 - kWarps * kSlots * (D + 2) * 4) / (kWarps * kStageBytes));
-  static constexpr int kRing = kWarps * kStages * kStageBytes;
-  static constexpr int kSmem = 1024 + kRing + kWarps * kSlots * (D + 2) * 4 + kWarps * kStages * 8;
-  static_assert(kStages >= 2, "ring too small");
+  static constexpr int kWarps = NT == 1 ? 12 : 8;
+  static constexpr int kStages = std::min(6, 222 * 1024 / (kWarps * kStageBytes));
+  static constexpr int kSmem = 1024 + kWarps * kStages * (kStageBytes + 8);
+  static_assert(kStages >= 2 && kSmem <= 226 * 1024, "ring");
 };
 
-// Tiles per (head block) row block: rows and q heads that share kSlots slots.
+// Rows and q heads that share an item's slots.
 __host__ __device__ inline void block_shape(int slots, int ratio, int &rb, int &hb, int &head_blocks) {
   hb = min(ratio, slots);
   rb = max(1, slots / ratio);
@@ -247,23 +267,21 @@ __host__ __device__ inline void block_shape(int slots, int ratio, int &rb, int &
 }
 
 template <typename T, int BITS, int D, int NT>
-__global__ void __launch_bounds__(32 * kWarps, Shape<T, BITS, D, NT>::kCtas)
+__global__ void __launch_bounds__(32 * Shape<T, BITS, D, NT>::kWarps, 1)
     attend_kernel(const __grid_constant__ AttendArgs a) {
   using S = Shape<T, BITS, D, NT>;
-  constexpr int G = S::kGroups, SL = S::kSlots;
+  constexpr int G = S::kGroups, SL = S::kSlots, W = S::kWarps;
   constexpr bool SPLIT = S::kSplit;
-  constexpr int kSteps = D / 16;  // K steps of the score product
+  constexpr int NS = SPLIT ? 1 : 2;  // slots of a lane's two columns
+  constexpr int kSteps = D / 16;     // K steps of the score product
+  constexpr int kTile = S::kTile;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float *buf = reinterpret_cast<float *>(smem + S::kRing);  // [warp][slot][D + 2]
-  uint64_t *bars = reinterpret_cast<uint64_t *>(buf + kWarps * SL * (D + 2));
-  __shared__ long long s_scan[kWarps];
-  __shared__ long long s_at;  // tiles before the first segment of this CTA's range
-  __shared__ int s_seg;
+  __shared__ long long s_before[32 * W], s_scan[W];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
   uint8_t *ring = smem + warp * S::kStages * S::kStageBytes;
-  uint64_t *full = bars + warp * S::kStages;
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + W * S::kStages * S::kStageBytes) + warp * S::kStages;
   if (lane == 0) {
     for (int i = 0; i < S::kStages; ++i) mbar_init(&full[i], 1);
     fence_mbar_init();
@@ -274,69 +292,69 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<T, BITS, D, NT>::kCtas)
   pdl_wait();  // cache, queries and rows may be written by the previous kernel
   pdl_trigger();
 
-  // ---- this CTA's range of the list of tiles
-  const int each = (a.rows.segments + 32 * kWarps - 1) / (32 * kWarps);
-  const int b_lo = min(tid * each, a.rows.segments), b_hi = min(b_lo + each, a.rows.segments);
+  // ---- the list of tiles: thread t counts segments [t each, (t + 1) each)
+  const int each = (a.rows.segments + 32 * W - 1) / (32 * W);
   long long mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) mine += load_segment<kTile>(a.rows, b, rb).units * per_seg;
-  long long before = mine;  // inclusive prefix over the threads
+  for (int b = tid * each; b < min((tid + 1) * each, a.rows.segments); ++b)
+    mine += load_segment<kTile>(a.rows, b, rb).units * per_seg;
+  long long before = mine;  // inclusive prefix over the warp's threads
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const long long x = __shfl_up_sync(0xffffffffu, before, o);
     if (lane >= o) before += x;
   }
   if (lane == 31) s_scan[warp] = before;
+  s_before[tid] = before - mine;
   __syncthreads();
-  long long total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += s_scan[w];
-    total += s_scan[w];
+  long long total = 0, base = 0;  // base: tiles counted by earlier warps
+  for (int w = 0; w < W; ++w) {
+    const long long x = s_scan[w];
+    total += x;
+    if (w < warp) base += x;
   }
-  before -= mine;
-  // every CTA with work has a tile for each warp
-  const long long ctas = min((long long)gridDim.x, max(1ll, (total + kWarps - 1) / kWarps));
-  const long long c = blockIdx.x;
-  const long long u0 = c < ctas ? c * total / ctas : 0, u1 = c < ctas ? (c + 1) * total / ctas : 0;
-  int *desc = a.desc + (size_t)c * 2 * kDescWords;
-  if (tid == 0) desc[0] = desc[kDescWords] = 0;
+  s_before[tid] += base;
+  __syncthreads();
+  // ---- this warp's range: with few tiles, one each to the first warps of all CTAs
+  const long long workers = max(1ll, min((long long)gridDim.x * W, total)), me = (long long)warp * gridDim.x + blockIdx.x;
+  const long long u0 = me < workers ? me * total / workers : 0, u1 = me < workers ? (me + 1) * total / workers : 0;
+  int *desc = a.desc + me * kDescWords;
+  if (lane == 0) desc[0] = 0;
   if (u0 >= u1) return;
-  if (before <= u0 && u0 < before + mine) {
-    long long at = before;
-    for (int b = b_lo; b < b_hi; ++b) {
-      const long long n = load_segment<kTile>(a.rows, b, rb).units * per_seg;
-      if (u0 < at + n) {
-        s_seg = b;
-        s_at = at;
-        break;
-      }
-      at += n;
-    }
-  }
-  __syncthreads();
-  int b = s_seg;
-  long long seg_at = s_at;
+  int at = 0;  // the last thread whose count starts at or before u0
+  for (int i = lane; i < 32 * W; i += 32) at += s_before[i] <= u0;
+  at = __reduce_add_sync(0xffffffffu, at) - 1;
+  // (threads past the last segment start at `total`; equal starts are segments without rows)
+  int b = at * each;
+  long long seg_at = s_before[at];
   Segment sg = load_segment<kTile>(a.rows, b, rb);
-  long long u = u0;
-  unsigned issued = 0, used = 0;  // ring positions of this warp
-  bool dead = false;              // a wait ran out
 
-  while (u < u1) {
+  const Decode dec(BITS);
+  const uint64_t pol = l2_policy_evict_first();
+  // this lane's ldmatrix address within 16 positions (position lane % 16, chunk lane / 16)
+  constexpr int kPerLine = 128 / S::kRowBytes;
+  const int lr = lane & 15;
+  const uint32_t frag = (lr / kPerLine) * 128 +
+                        ((((lr % kPerLine) * S::kChunks + (lane >> 4)) ^ ((lr / kPerLine) & 7)) << 4);
+  unsigned issued = 0, used = 0;  // ring positions
+  bool dead = false;              // a wait ran out
+  long long u = u0;
+
+  while (u < u1 && !dead) {
     while (u >= seg_at + sg.units * per_seg) {
       seg_at += sg.units * per_seg;
       sg = load_segment<kTile>(a.rows, ++b, rb);
     }
-    // item: K/V head h, head block, row block cb, tiles [t_lo, t_hi) of its `tiles`
+    // ---- item: K/V head h, q heads from head0, row block cb, tiles [t_lo, t_hi) of `tiles`
     const long long in_seg = u - seg_at;
     const int hh = (int)(in_seg / sg.units), h = hh / head_blocks, head0 = (hh - h * head_blocks) * hb;
     const long long in_head = in_seg - (long long)hh * sg.units;
-    int lo = 0, hi = sg.blocks;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (block_prefix<kTile>(sg, rb, mid) <= in_head) lo = mid;
+    int cb = 0;
+    for (int hi = sg.blocks; hi - cb > 1;) {
+      const int mid = (cb + hi) >> 1;
+      if (block_prefix<kTile>(sg, rb, mid) <= in_head) cb = mid;
       else hi = mid;
     }
-    const int cb = lo, row0 = cb * rb;
+    const int row0 = cb * rb;
     const int ok_rows = max(0, min(rb, sg.ok_rows - row0));  // rows of this block in range
     const int nrows = min(rb, sg.n - row0);
     const int len = ok_rows > 0 ? sg.start + row0 + ok_rows : 0;
@@ -344,39 +362,39 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<T, BITS, D, NT>::kCtas)
     const long long item_u0 = seg_at + (long long)hh * sg.units + block_prefix<kTile>(sg, rb, cb);
     const int t_lo = (int)(u - item_u0), t_hi = (int)min((long long)tiles, u1 - item_u0);
     u = item_u0 + t_hi;
-    const int nt = len > 0 ? t_hi - t_lo : 0;                    // tiles to read
-    const int my = nt > warp ? (nt - warp + kWarps - 1) / kWarps : 0;  // of this warp
-    const size_t srow = ((size_t)h * (size_t)a.capacity);
-    const __nv_bfloat16 *ks_g = a.k_scales + (size_t)(len ? sg.seq : 0) * (size_t)a.scale_seq_stride + srow * G;
-    const __nv_bfloat16 *vs_g = a.v_scales + (size_t)(len ? sg.seq : 0) * (size_t)a.scale_seq_stride + srow * G;
-    auto issue = [&](int i) {  // the warp's i-th tile of the item (lane 0)
-      const int st = issued % S::kStages, pos = (t_lo + warp + i * kWarps) * kTile;
+    const int nt = len > 0 ? t_hi - t_lo : 0;  // tiles to read
+    const size_t sc_at =
+        (size_t)(len ? sg.seq : 0) * (size_t)a.scale_seq_stride + (size_t)h * (size_t)a.capacity * G;
+    auto issue = [&](int i) {  // the i-th tile of the item (lane 0)
+      const int st = issued % S::kStages, pos = (t_lo + i) * kTile;
       uint8_t *dst = ring + st * S::kStageBytes;
       mbar_arrive_expect_tx(&full[st], S::kTxBytes);
-      tma_load_4d(dst, &a.k_map, 0, pos, h, sg.seq, &full[st]);
-      tma_load_4d(dst + S::kCodeBytes, &a.v_map, 0, pos, h, sg.seq, &full[st]);
-      const uint64_t pol = l2_policy_evict_first();
-      bulk_g2s(dst + 2 * S::kCodeBytes, ks_g + (size_t)pos * G, S::kScaleBytes, &full[st], pol);
-      bulk_g2s(dst + 2 * S::kCodeBytes + S::kScaleBytes, vs_g + (size_t)pos * G, S::kScaleBytes, &full[st], pol);
+      tma_load_4d(dst, &a.k_map, 0, pos / kPerLine, h, sg.seq, &full[st]);
+      tma_load_4d(dst + S::kCodeBytes, &a.v_map, 0, pos / kPerLine, h, sg.seq, &full[st]);
+      bulk_g2s(dst + 2 * S::kCodeBytes, a.k_scales + sc_at + (size_t)pos * G, S::kScaleBytes, &full[st], pol);
+      bulk_g2s(dst + 2 * S::kCodeBytes + S::kScaleBytes, a.v_scales + sc_at + (size_t)pos * G, S::kScaleBytes,
+               &full[st], pol);
     };
-    int ahead = dead ? 0 : min(my, S::kStages);
-    for (int i = 0; i < ahead; ++i) {
+    for (int i = 0; i < min(nt, S::kStages); ++i) {
       if (lane == 0) issue(i);
       ++issued;
     }
 
     // ---- queries: the B operand of the score product, column n = gid
     unsigned qb[NT][kSteps][2];
-    float cmul[NT][2];  // score factor of columns 2 tig, 2 tig + 1
-    int lim[NT][2];                     // positions that the slot's row sees
-    auto slot_row = [&](int slot) { return slot / hb; };
+    float cmul[NT][NS];  // score factor of this lane's slots
+    int lim[NT][NS];     // positions that the slot's row sees
+    auto slot_stored = [&](int slot) {
+      return slot < rb * hb && slot / hb < nrows && head0 + slot % hb < a.ratio;
+    };
     auto slot_limit = [&](int slot) {
-      const int i = slot_row(slot);
-      if (i >= nrows || slot >= rb * hb) return len;  // no row: never masked, never stored
+      const int i = slot / hb;
+      if (i >= nrows || slot >= rb * hb) return len;  // no row: never stored
       return i < ok_rows ? sg.start + row0 + i + 1 : 0;
     };
-    auto slot_stored = [&](int slot) {
-      return slot < rb * hb && slot_row(slot) < nrows && head0 + slot % hb < a.ratio;
+    auto slot_offset = [&](int slot, long long row_stride, long long head_stride) {
+      return (size_t)(sg.r0 + row0 + slot / hb) * (size_t)row_stride +
+             (size_t)(h * a.ratio + head0 + slot % hb) * (size_t)head_stride;
     };
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -384,9 +402,8 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<T, BITS, D, NT>::kCtas)
       const bool lo_half = SPLIT && (gid & 1);
       float x[kSteps][4];
       float top = 0.f;
-      const T *qp = static_cast<const T *>(a.q) + (size_t)(sg.r0 + row0 + slot_row(slot)) * (size_t)a.q_row +
-                    (size_t)(h * a.ratio + head0 + slot % hb) * (size_t)a.q_head;
-      const bool have = slot_stored(slot) && slot_row(slot) < ok_rows;
+      const T *qp = static_cast<const T *>(a.q) + slot_offset(slot, a.q_row, a.q_head);
+      const bool have = slot_stored(slot) && slot / hb < ok_rows;
       if constexpr (BITS == 4) {
         // word tig of group g: dimensions 32 g + 8 tig + (0 .. 7)
 #pragma unroll
@@ -424,7 +441,9 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<T, BITS, D, NT>::kCtas)
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       // scale the row so that its largest element lies in [2^12, 2^13)
       const int fe = min(254, 266 - (int)((__float_as_uint(top) >> 23) & 255u));
-      const float f = __uint_as_float((unsigned)fe << 23), finv = __uint_as_float((unsigned)(254 - fe) << 23);
+      // (with the softmax scale's sign, so that the factor of the products is > 0)
+      const float f = copysignf(__uint_as_float((unsigned)fe << 23), a.scale_log2);
+      const float finv = __uint_as_float((unsigned)(254 - fe) << 23);
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         float y[4];
@@ -437,16 +456,13 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<T, BITS, D, NT>::kCtas)
         qb[t][s][1] = pack_f16(y[2], y[3]);
       }
       // column n's factor sits in lanes 4 n ..; the accumulators hold columns 2 tig, 2 tig + 1
-      const float cm = a.scale_log2 * finv;
-      cmul[t][0] = __shfl_sync(0xffffffffu, cm, 8 * tig);
-      cmul[t][1] = __shfl_sync(0xffffffffu, cm, 8 * tig + 4);
-      lim[t][0] = slot_limit(SPLIT ? 4 * t + tig : 8 * t + 2 * tig);
-      lim[t][1] = SPLIT ? lim[t][0] : slot_limit(8 * t + 2 * tig + 1);
+      const float cm = fmaxf(fabsf(a.scale_log2) * finv, 1e-37f);
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        cmul[t][i] = __shfl_sync(0xffffffffu, cm, 8 * tig + 4 * i);
+        lim[t][i] = slot_limit(SPLIT ? 4 * t + tig : 8 * t + 2 * tig + i);
+      }
     }
-    // positions below this are seen by every row of the block
-    const int seen_by_all = ok_rows == nrows ? len - ok_rows + 1 : 0;
-
-    constexpr int NS = SPLIT ? 1 : 2;  // slots of a lane's two columns
     float m[NT][NS], l[NT][NS];
     float acc[NT][G][2][4];
 #pragma unroll
@@ -462,227 +478,228 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<T, BITS, D, NT>::kCtas)
         for (int i = 0; i < 4; ++i) acc[t][g][0][i] = acc[t][g][1][i] = 0.f;
     }
 
-    auto tile_step = [&](int pos0, const uint8_t *st, auto masked) {
-      constexpr bool MASK = decltype(masked)::value;
-      const uint32_t kb = smem_addr(st), vb = kb + S::kCodeBytes;
-      const uint8_t *ksc = st + 2 * S::kCodeBytes, *vsc = ksc + S::kScaleBytes;
-      // row of this lane's ldmatrix address within 16 positions, and its swizzle
-      const int lr = lane & 15, lc = lane >> 4;
-      const int swz = S::kRowBytes == 128 ? (lr & 7) : S::kRowBytes == 64 ? ((lr >> 1) & 3) : ((lr >> 2) & 1);
-      float x[2][NT][2][NS];  // score [16 positions][tile][row gid, gid + 8][slot]
-#pragma unroll
-      for (int sub = 0; sub < 2; ++sub) {
-        float sc[2][G];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const uint8_t *p = ksc + (16 * sub + 8 * r + gid) * (G * 2);
-          if constexpr (G == 4) {
-            const uint2 w = *reinterpret_cast<const uint2 *>(p);
-            sc[r][0] = bf_lo(w.x), sc[r][1] = bf_hi(w.x), sc[r][2] = bf_lo(w.y), sc[r][3] = bf_hi(w.y);
-          } else {
-            const unsigned w = *reinterpret_cast<const unsigned *>(p);
-            sc[r][0] = bf_lo(w), sc[r][1] = bf_hi(w);
-          }
-        }
-        float s[NT][4];
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[t][i] = 0.f;
-#pragma unroll
-        for (int c2 = 0; c2 < S::kChunks; c2 += 2) {
-          unsigned w[4];  // chunk c2: rows gid, gid + 8; chunk c2 + 1: the same
-          ldmatrix4(w, kb + (16 * sub + lr) * S::kRowBytes + (((c2 + lc) ^ swz) << 4));
-          if constexpr (BITS == 4) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const int g = c2 + k;
-              unsigned ha[4], hs[4];  // rows gid, gid + 8
-              decode4(w[2 * k], ha);
-              decode4(w[2 * k + 1], hs);
-#pragma unroll
-              for (int t = 0; t < NT; ++t) {
-                float cc[4];
-                mma_f16(cc, ha[0], hs[0], ha[1], hs[1], qb[t][2 * g][0], qb[t][2 * g][1], 0.f, 0.f, 0.f, 0.f);
-                mma_acc(cc, ha[2], hs[2], ha[3], hs[3], qb[t][2 * g + 1][0], qb[t][2 * g + 1][1]);
-                s[t][0] = fmaf(sc[0][g], cc[0], s[t][0]);
-                s[t][1] = fmaf(sc[0][g], cc[1], s[t][1]);
-                s[t][2] = fmaf(sc[1][g], cc[2], s[t][2]);
-                s[t][3] = fmaf(sc[1][g], cc[3], s[t][3]);
-              }
-            }
-          } else {
-            const int g = c2 / 2;
-            unsigned h[4][2];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) decode8(w[k], h[k]);
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              float cc[4];
-              mma_f16(cc, h[0][0], h[1][0], h[0][1], h[1][1], qb[t][c2][0], qb[t][c2][1], 0.f, 0.f, 0.f, 0.f);
-              mma_acc(cc, h[2][0], h[3][0], h[2][1], h[3][1], qb[t][c2 + 1][0], qb[t][c2 + 1][1]);
-              s[t][0] = fmaf(sc[0][g], cc[0], s[t][0]);
-              s[t][1] = fmaf(sc[0][g], cc[1], s[t][1]);
-              s[t][2] = fmaf(sc[1][g], cc[2], s[t][2]);
-              s[t][3] = fmaf(sc[1][g], cc[3], s[t][3]);
-            }
-          }
-        }
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            if constexpr (SPLIT) {
-              x[sub][t][r][0] = (s[t][2 * r] + s[t][2 * r + 1]) * cmul[t][0];
-            } else {
-              x[sub][t][r][0] = s[t][2 * r] * cmul[t][0];
-              x[sub][t][r][1] = s[t][2 * r + 1] * cmul[t][1];
-            }
-          }
-      }
-      // V scales of this lane's 4 positions, and the exponent of the tile's largest
-      uint2 vw[2][2];
-      unsigned vmax = 0;
-#pragma unroll
-      for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int row = 16 * sub + 8 * r + gid;
-          if constexpr (G == 4) vw[sub][r] = *reinterpret_cast<const uint2 *>(vsc + row * 8);
-          else vw[sub][r] = make_uint2(*reinterpret_cast<const unsigned *>(vsc + row * 4), 0u);
-          if (MASK && pos0 + row >= len) vw[sub][r] = make_uint2(0u, 0u);
-          vmax = __vmaxu2(vmax, __vmaxu2(vw[sub][r].x, vw[sub][r].y));
-        }
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) vmax = __vmaxu2(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
-      // 2^40 either way: beyond it p s leaves fp16's range or the sum of p underflows
-      const int ve = min(max((int)(max(vmax & 0xffffu, vmax >> 16) >> 7), 127 - 40), 127 + 40);
-      const float vinv = __uint_as_float((unsigned)(254 - ve) << 23), vexp = (float)(ve - 127);
-      float corr[NT][NS];
-      bool moved = false;
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int i = 0; i < NS; ++i) {
-          float mx = m[t][i];
-#pragma unroll
-          for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              float &y = x[sub][t][r][i];
-              y += vexp;
-              if (MASK && pos0 + 16 * sub + 8 * r + gid >= lim[t][i]) y = -INFINITY;
-              mx = fmaxf(mx, y);
-            }
-#pragma unroll
-          for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-          const float ref = (mx == -INFINITY ? 0.f : mx) - kShift;  // (-inf: nothing seen yet)
-          corr[t][i] = fast_exp2(m[t][i] - (ref + kShift));
-          moved |= mx != m[t][i];
-          m[t][i] = mx;
-          float sum = 0.f;
-#pragma unroll
-          for (int sub = 0; sub < 2; ++sub)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              x[sub][t][r][i] = fast_exp2(x[sub][t][r][i] - ref);
-              sum += x[sub][t][r][i];
-            }
-          l[t][i] = l[t][i] * corr[t][i] + sum * vinv;
-        }
-      if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int g = 0; g < G; ++g)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float cr = corr[t][NS == 1 ? 0 : (i & 1)];
-              acc[t][g][0][i] *= cr;
-              acc[t][g][1][i] *= cr;
-            }
-      }
-      // outputs
-#pragma unroll
-      for (int sub = 0; sub < 2; ++sub) {
-        float sv[2][4];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          sv[r][0] = bf_lo(vw[sub][r].x) * vinv;
-          sv[r][1] = bf_hi(vw[sub][r].x) * vinv;
-          sv[r][2] = bf_lo(vw[sub][r].y) * vinv;
-          sv[r][3] = bf_hi(vw[sub][r].y) * vinv;
-        }
-        auto p_frag = [&](int t, int g, unsigned (&pb)[2]) {
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            float y0 = x[sub][t][r][0] * sv[r][g], y1;
-            if (MASK && x[sub][t][r][0] == 0.f) y0 = 0.f;  // whatever the scale holds
-            if constexpr (SPLIT) {
-              y1 = y0 - f16_round(y0);
-            } else {
-              y1 = x[sub][t][r][1] * sv[r][g];
-              if (MASK && x[sub][t][r][1] == 0.f) y1 = 0.f;
-            }
-            pb[r] = transpose8(pack_f16(y0, y1));
-          }
-        };
-#pragma unroll
-        for (int c2 = 0; c2 < S::kChunks; c2 += 2) {
-          unsigned w[4];  // chunk c2: positions 0-7, 8-15; chunk c2 + 1: the same
-          // lanes 0-15 address the positions of chunk c2, lanes 16-31 of c2 + 1
-          ldmatrix4_trans(w, vb + (16 * sub + lr) * S::kRowBytes + (((c2 + lc) ^ swz) << 4));
-          if constexpr (BITS == 4) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const int g = c2 + k;
-              unsigned ha[4], hs[4];  // positions 0-7, 8-15
-              decode4(w[2 * k], ha);
-              decode4(w[2 * k + 1], hs);
-#pragma unroll
-              for (int t = 0; t < NT; ++t) {
-                unsigned pb[2];
-                p_frag(t, g, pb);
-                mma_acc(acc[t][g][0], ha[0], ha[1], hs[0], hs[1], pb[0], pb[1]);
-                mma_acc(acc[t][g][1], ha[2], ha[3], hs[2], hs[3], pb[0], pb[1]);
-              }
-            }
-          } else {
-            const int g = c2 / 2;
-            unsigned h[4][2];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) decode8(w[k], h[k]);
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              unsigned pb[2];
-              p_frag(t, g, pb);
-              mma_acc(acc[t][g][0], h[0][0], h[0][1], h[1][0], h[1][1], pb[0], pb[1]);
-              mma_acc(acc[t][g][1], h[2][0], h[2][1], h[3][0], h[3][1], pb[0], pb[1]);
-            }
-          }
-        }
-      }
-    };
-
-    for (int i = 0; i < my && !dead; ++i) {
+    for (int i = 0; i < nt; ++i) {
       const int st = used % S::kStages;
       if (!__all_sync(0xffffffffu, wait_copy(&full[st], (used / S::kStages) & 1))) {
         dead = true;
         break;
       }
       ++used;
-      const int pos0 = (t_lo + warp + i * kWarps) * kTile;
-      const uint8_t *stage = ring + st * S::kStageBytes;
-      if (pos0 + kTile <= seen_by_all) tile_step(pos0, stage, std::false_type{});
-      else tile_step(pos0, stage, std::true_type{});
+      const int pos0 = (t_lo + i) * kTile;
+      uint8_t *stage = ring + st * S::kStageBytes;
+      if (pos0 + kTile > len) {
+        // the scales of positions that no row sees may hold anything: zero
+        for (int p = (len - pos0) * G + lane; p < kTile * G; p += 32) {
+          reinterpret_cast<__nv_bfloat16 *>(stage + 2 * S::kCodeBytes)[p] = __float2bfloat16_rn(0.f);
+          reinterpret_cast<__nv_bfloat16 *>(stage + 2 * S::kCodeBytes + S::kScaleBytes)[p] = __float2bfloat16_rn(0.f);
+        }
+        fence_proxy_async_smem();  // before a later copy into this stage
+        __syncwarp();
+      }
+#pragma unroll 1
+      for (int half = 0; half < kTile / 32; ++half) {  // 32 positions
+        const int p0 = 32 * half;
+        const uint32_t kb = smem_addr(stage) + p0 * S::kRowBytes, vb = kb + S::kCodeBytes;
+        const uint8_t *ksc = stage + 2 * S::kCodeBytes + (p0 + gid) * (G * 2), *vsc = ksc + S::kScaleBytes;
+        // products q . k over the factor cmul: [16 positions][tile][row gid, gid + 8][slot]; then p
+        float x[2][NT][2][NS];
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
+          float sc[2][G];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const uint8_t *p = ksc + (16 * sub + 8 * r) * (G * 2);
+            if constexpr (G == 4) {
+              const uint2 w = *reinterpret_cast<const uint2 *>(p);
+              sc[r][0] = bf_lo(w.x), sc[r][1] = bf_hi(w.x), sc[r][2] = bf_lo(w.y), sc[r][3] = bf_hi(w.y);
+            } else {
+              const unsigned w = *reinterpret_cast<const unsigned *>(p);
+              sc[r][0] = bf_lo(w), sc[r][1] = bf_hi(w);
+            }
+          }
+          float s[NT][4];
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)  // what the slot's row does not see starts from -inf
+              s[t][k] = pos0 + p0 + 16 * sub + 8 * (k >> 1) + gid < lim[t][SPLIT ? 0 : (k & 1)] ? 0.f : -INFINITY;
+#pragma unroll
+          for (int c2 = 0; c2 < S::kChunks; c2 += 2) {
+            unsigned w[4];  // chunk c2: rows gid, gid + 8; chunk c2 + 1: the same
+            ldmatrix4(w, (kb + 16 * sub * S::kRowBytes + frag) ^ ((c2 ^ (kPerLine == 4 ? 4 * (sub & 1) : 0)) << 4));
+            if constexpr (BITS == 4) {
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const int g = c2 + k;
+                unsigned ha[4], hs[4];  // rows gid, gid + 8
+                dec.nibbles(w[2 * k], ha);
+                dec.nibbles(w[2 * k + 1], hs);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                  float cc[4];
+                  mma_f16(cc, ha[0], hs[0], ha[1], hs[1], qb[t][2 * g][0], qb[t][2 * g][1], 0.f, 0.f, 0.f, 0.f);
+                  mma_acc(cc, ha[2], hs[2], ha[3], hs[3], qb[t][2 * g + 1][0], qb[t][2 * g + 1][1]);
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) s[t][e] = fmaf(sc[e >> 1][g], cc[e], s[t][e]);
+                }
+              }
+            } else {
+              const int g = c2 / 2;
+              unsigned hd[4][2];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) dec.bytes(w[k], hd[k]);
+#pragma unroll
+              for (int t = 0; t < NT; ++t) {
+                float cc[4];
+                mma_f16(cc, hd[0][0], hd[1][0], hd[0][1], hd[1][1], qb[t][c2][0], qb[t][c2][1], 0.f, 0.f, 0.f, 0.f);
+                mma_acc(cc, hd[2][0], hd[3][0], hd[2][1], hd[3][1], qb[t][c2 + 1][0], qb[t][c2 + 1][1]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[t][e] = fmaf(sc[e >> 1][g], cc[e], s[t][e]);
+              }
+            }
+          }
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              if constexpr (SPLIT) {
+                x[sub][t][r][0] = s[t][2 * r] + s[t][2 * r + 1];
+              } else {
+                x[sub][t][r][0] = s[t][2 * r];
+                x[sub][t][r][1] = s[t][2 * r + 1];
+              }
+            }
+        }
+        // V scales of this lane's positions, and the exponent of the largest
+        uint2 vw[2][2];
+        unsigned vmax = 0;
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const uint8_t *p = vsc + (16 * sub + 8 * r) * (G * 2);
+            if constexpr (G == 4) vw[sub][r] = *reinterpret_cast<const uint2 *>(p);
+            else vw[sub][r] = make_uint2(*reinterpret_cast<const unsigned *>(p), 0u);
+            vmax = max_u16x2(vmax, max_u16x2(vw[sub][r].x, vw[sub][r].y));
+          }
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) vmax = max_u16x2(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
+        // 2^40 either way: beyond it p s leaves fp16's range or p leaves fp32's
+        const int ve = min(max((int)(max(vmax & 0xffffu, vmax >> 16) >> 7), 127 - 40), 127 + 40);
+        const float vexp = (float)(ve - 127);
+        float corr[NT][NS];
+        bool moved = false;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int i = 0; i < NS; ++i) {
+            float mx = fmaxf(fmaxf(x[0][t][0][i], x[0][t][1][i]), fmaxf(x[1][t][0][i], x[1][t][1][i]));
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            // m: running maximum of score + e; -inf: nothing seen yet
+            const float mn = fmaxf(m[t][i], fmaf(mx, cmul[t][i], vexp));
+            const float ref = mn == -INFINITY ? 0.f : mn;
+            corr[t][i] = fast_exp2(m[t][i] - ref);
+            moved |= mn != m[t][i];
+            m[t][i] = mn;
+            float sum = 0.f;
+#pragma unroll
+            for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                x[sub][t][r][i] = fast_exp2(fmaf(x[sub][t][r][i], cmul[t][i], kShift - ref));
+                sum += x[sub][t][r][i];
+              }
+            l[t][i] = fmaf(l[t][i], corr[t][i], sum);
+          }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float cr = corr[t][NS == 1 ? 0 : (e & 1)];
+                acc[t][g][0][e] *= cr;
+                acc[t][g][1][e] *= cr;
+              }
+        }
+        // outputs
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
+          float sv[2][4];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            sv[r][0] = bf_lo(vw[sub][r].x);
+            sv[r][1] = bf_hi(vw[sub][r].x);
+            sv[r][2] = bf_lo(vw[sub][r].y);
+            sv[r][3] = bf_hi(vw[sub][r].y);
+          }
+          auto p_frag = [&](int t, int g, unsigned (&pb)[2]) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const float y0 = x[sub][t][r][0] * sv[r][g];
+              const float y1 = SPLIT ? y0 - f16_round(y0) : x[sub][t][r][NS - 1] * sv[r][g];
+              pb[r] = transpose8(pack_f16(y0, y1));
+            }
+          };
+#pragma unroll
+          for (int c2 = 0; c2 < S::kChunks; c2 += 2) {
+            unsigned w[4];  // chunk c2: positions 0-7, 8-15; chunk c2 + 1: the same
+            ldmatrix4_trans(w,
+                            (vb + 16 * sub * S::kRowBytes + frag) ^ ((c2 ^ (kPerLine == 4 ? 4 * (sub & 1) : 0)) << 4));
+            if constexpr (BITS == 4) {
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const int g = c2 + k;
+                unsigned ha[4], hs[4];  // positions 0-7, 8-15
+                dec.nibbles(w[2 * k], ha);
+                dec.nibbles(w[2 * k + 1], hs);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                  unsigned pb[2];
+                  p_frag(t, g, pb);
+                  mma_acc(acc[t][g][0], ha[0], ha[1], hs[0], hs[1], pb[0], pb[1]);
+                  mma_acc(acc[t][g][1], ha[2], ha[3], hs[2], hs[3], pb[0], pb[1]);
+                }
+              }
+            } else {
+              const int g = c2 / 2;
+              unsigned hd[4][2];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) dec.bytes(w[k], hd[k]);
+#pragma unroll
+              for (int t = 0; t < NT; ++t) {
+                unsigned pb[2];
+                p_frag(t, g, pb);
+                mma_acc(acc[t][g][0], hd[0][0], hd[0][1], hd[1][0], hd[1][1], pb[0], pb[1]);
+                mma_acc(acc[t][g][1], hd[2][0], hd[2][1], hd[3][0], hd[3][1], pb[0], pb[1]);
+              }
+            }
+          }
+        }
+      }
       __syncwarp();  // every lane has read the stage
-      if (i + S::kStages < my) {
+      if (i + S::kStages < nt) {
         if (lane == 0) issue(i + S::kStages);
         ++issued;
       }
     }
 
-    // ---- the warp's state to shared memory: per slot m, l, outputs
+    // ---- the item's rows, or the part of them that this range holds
+    const bool whole = t_lo == 0 && t_hi == tiles, head_part = t_lo == 0;
+    if (lane == 0) {
+      if (!whole && head_part) {
+        desc[1] = sg.r0 + row0;
+        desc[2] = nrows;
+        desc[3] = h * a.ratio + head0;
+        desc[4] = min(hb, a.ratio - head0);
+        // parts: this worker's and those up to the worker with the item's last tile
+        desc[0] = (int)(((item_u0 + tiles) * workers - 1) / total - me) + 1;
+      }
+      if (ok_rows < nrows && a.status) atomicOr(a.status, QMK_KV_BAD_ROW);
+    }
+    float *part = a.parts + (size_t)(me * 2 + (head_part ? 0 : 1)) * SL * (D + 4);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -690,146 +707,143 @@ __global__ void __launch_bounds__(32 * kWarps, Shape<T, BITS, D, NT>::kCtas)
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) l[t][i] += __shfl_xor_sync(0xffffffffu, l[t][i], o);
         const int slot = SPLIT ? 4 * t + tig : 8 * t + 2 * tig + i;
-        float *dst = buf + (warp * SL + slot) * (D + 2);
-        if (gid == 0) *reinterpret_cast<float2 *>(dst + D) = make_float2(m[t][i], l[t][i]);
+        if (!slot_stored(slot)) continue;
+        const float inv = whole ? (l[t][i] == 0.f ? 0.f : 1.f / l[t][i]) : 1.f;  // 0: the row sees nothing
+        float *dst = part + slot * (D + 4);
+        T *o = static_cast<T *>(a.out) + slot_offset(slot, a.o_row, a.o_head);
+        if (!whole && gid == 0) *reinterpret_cast<float2 *>(dst + D) = make_float2(m[t][i], l[t][i]);
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-          float y[2][2];  // [product][row gid, gid + 8]
+        for (int g = 0; g < G; ++g)
 #pragma unroll
-          for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const float *v = &acc[t][g][k][2 * r];
-              y[k][r] = SPLIT ? v[0] + v[1] : v[i];
+          for (int k = 0; k < 2; ++k) {
+            // 4 bits: dimensions 32 g + 4 gid + 2 k + (0, 1); 8 bits: 32 g + 16 k + 2 gid + (0, 1)
+            const int d = 32 * g + (BITS == 4 ? 4 * gid + 2 * k : 16 * k + 2 * gid);
+            const float *v = acc[t][g][k];
+            const float y0 = (SPLIT ? v[0] + v[1] : v[i]) * inv, y1 = (SPLIT ? v[2] + v[3] : v[2 + i]) * inv;
+            if (whole) {
+              o[d] = from_float<T>(y0);
+              o[d + 1] = from_float<T>(y1);
+            } else {
+              *reinterpret_cast<float2 *>(dst + d) = make_float2(y0, y1);
             }
-          if constexpr (BITS == 4) {  // dimensions 32 g + 4 gid + 2 k + r
-            *reinterpret_cast<float2 *>(dst + 32 * g + 4 * gid) = make_float2(y[0][0], y[0][1]);
-            *reinterpret_cast<float2 *>(dst + 32 * g + 4 * gid + 2) = make_float2(y[1][0], y[1][1]);
-          } else {  // dimensions 32 g + 16 k + 2 gid + r
-            *reinterpret_cast<float2 *>(dst + 32 * g + 2 * gid) = make_float2(y[0][0], y[0][1]);
-            *reinterpret_cast<float2 *>(dst + 32 * g + 16 + 2 * gid) = make_float2(y[1][0], y[1][1]);
           }
-        }
       }
     }
-    if (dead && lane == 0) {
-      if (a.status) atomicOr(a.status, QMK_KV_TIMEOUT);
-      // copies in flight must land before this shared memory is reused
-      bool drained = true;
-      for (; used != issued; ++used) drained &= wait_copy(&full[used % S::kStages], (used / S::kStages) & 1);
-      if (!drained && a.status) atomicOr(a.status, QMK_KV_COPIES_PENDING);
-    }
-    if (dead) used = issued;
-    __syncthreads();
-    // ---- the warps' states joined; slot by slot, a warp a slot
-    const bool whole = t_lo == 0 && t_hi == tiles, head_part = t_lo == 0;
-    if (!whole && tid == 0) {
-      int *dd = desc + (head_part ? kDescWords : 0);
-      dd[0] = 1;
-      dd[1] = sg.r0 + row0;
-      dd[2] = nrows;
-      dd[3] = h * a.ratio + head0;
-      dd[4] = min(hb, a.ratio - head0);
-      // parts: this CTA's and those of the CTAs up to the one with the item's last tile
-      dd[5] = (int)(((item_u0 + tiles) * ctas - 1) / total - c) + 1;
-    }
-    if (ok_rows < nrows && tid == 0 && a.status) atomicOr(a.status, QMK_KV_BAD_ROW);
-    float *part = a.parts + ((size_t)c * 2 + (head_part ? 1 : 0)) * SL * (D + 2);
-    for (int slot = warp; slot < SL; slot += kWarps) {
-      if (!slot_stored(slot)) continue;
-      float M = -INFINITY, L = 0.f;
-      float w[kWarps];
-#pragma unroll
-      for (int k = 0; k < kWarps; ++k) M = fmaxf(M, buf[(k * SL + slot) * (D + 2) + D]);
-#pragma unroll
-      for (int k = 0; k < kWarps; ++k) {
-        const float mk = buf[(k * SL + slot) * (D + 2) + D];
-        w[k] = mk == -INFINITY ? 0.f : fast_exp2(mk - M);
-        L += w[k] * buf[(k * SL + slot) * (D + 2) + D + 1];
-      }
-      const float inv = whole ? (M == -INFINITY ? 0.f : 1.f / L) : 1.f;
-      constexpr int kPer = D / 32;
-      float y[kPer];
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) {
-        y[e] = 0.f;
-#pragma unroll
-        for (int k = 0; k < kWarps; ++k) y[e] += w[k] * buf[(k * SL + slot) * (D + 2) + 32 * e + lane];
-      }
-      if (whole) {
-        T *o = static_cast<T *>(a.out) + (size_t)(sg.r0 + row0 + slot_row(slot)) * (size_t)a.o_row +
-               (size_t)(h * a.ratio + head0 + slot % hb) * (size_t)a.o_head;
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) o[32 * e + lane] = from_float<T>(y[e] * inv);
-      } else {
-        float *p = part + slot * (D + 2);
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) p[32 * e + lane] = y[e];
-        if (lane == 0) *reinterpret_cast<float2 *>(p + D) = make_float2(M, L);
-      }
-    }
-    __syncthreads();  // buf is free again
+  }
+  if (dead && lane == 0) {
+    if (a.status) atomicOr(a.status, QMK_KV_TIMEOUT);
+    // copies in flight must land before this shared memory goes away
+    bool drained = true;
+    for (; used != issued; ++used) drained &= wait_copy(&full[used % S::kStages], (used / S::kStages) & 1);
+    if (!drained && a.status) atomicOr(a.status, QMK_KV_COPIES_PENDING);
   }
 }
 
-// Joins the parts of items that were cut: CTA c takes the item whose first
-// tile is in range c and that goes on in the next ranges; warp by slot.
+// Joins the parts of items that were cut: CTA c takes the items whose first
+// tile is in the range of worker c, c + grid, ... and that go on in the next
+// ranges.  A warp takes an output row, or several share one (few rows mean
+// many parts); 8 parts are loaded at a time.
+constexpr int kMergeWarps = 8;
+
 template <typename T, int D>
-__global__ void __launch_bounds__(128) merge_kernel(const int *__restrict__ desc, const float *__restrict__ parts,
-                                                    int slots, int hb, void *out, long long o_row, long long o_head) {
+__global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const int *__restrict__ desc,
+                                                                 const float *__restrict__ parts, int workers,
+                                                                 int slots, int hb, void *out, long long o_row,
+                                                                 long long o_head) {
   pdl_wait();  // the parts are written by attend_kernel
   pdl_trigger();
-  const int c = blockIdx.x;
-  const int *dd = desc + (size_t)c * 2 * kDescWords + kDescWords;
-  if (dd[0] == 0) return;
-  const int row0 = dd[1], nrows = dd[2], head0 = dd[3], nheads = dd[4], np = dd[5];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const size_t stride = (size_t)slots * (D + 2);
+  __shared__ float s_ml[kMergeWarps][2];
+  __shared__ float s_o[kMergeWarps][D];
   constexpr int kPer = D / 32;
-  for (int slot = warp; slot < slots; slot += 4) {
-    const int i = slot / hb, j = slot % hb;
-    if (i >= nrows || j >= nheads) continue;
-    // part k: CTA c + k's, the head part first
-    auto at = [&](int k) { return parts + ((size_t)(c + k) * 2 + (k == 0 ? 1 : 0)) * stride + (size_t)slot * (D + 2); };
-    float M = -INFINITY;
-    for (int k = lane; k < np; k += 32) M = fmaxf(M, at(k)[D]);
-    M = warp_max(M);
-    float L = 0.f, y[kPer];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int c = blockIdx.x; c < workers; c += gridDim.x) {
+    const int *dd = desc + (size_t)c * kDescWords;
+    const int np = dd[0];
+    if (np == 0) continue;
+    const int row0 = dd[1], nrows = dd[2], head0 = dd[3], nheads = dd[4], n = nrows * nheads;
+    const int share = n >= kMergeWarps ? 1 : kMergeWarps / n, at_once = kMergeWarps / share;  // warps a row, rows
+    for (int v0 = 0; v0 < n; v0 += at_once) {
+      const int v = v0 + warp / share, first = warp % share;
+      const bool live = v < n && warp < share * at_once;
+      const int i = live ? v / nheads : 0, j = live ? v % nheads : 0;
+      // part k: worker c + k's, the head part first
+      const float *p0 = parts + ((size_t)c * 2 * slots + i * hb + j) * (D + 4) + kPer * lane;
+      const size_t step = (size_t)2 * slots * (D + 4), tail = (size_t)slots * (D + 4);
+      float M = -INFINITY, L = 0.f, y[kPer];
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) y[e] = 0.f;
-    for (int k0 = 0; k0 < np; k0 += 32) {
-      float w = 0.f, lw = 0.f;
-      if (k0 + lane < np) {
-        const float2 ml = *reinterpret_cast<const float2 *>(at(k0 + lane) + D);
-        w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - M);
-        lw = w * ml.y;
+      for (int e = 0; e < kPer; ++e) y[e] = 0.f;
+      for (int k0 = first; live && k0 < np; k0 += 8 * share) {
+        float2 ml[8];
+        float x[8][kPer];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const int k = min(k0 + q * share, np - 1);
+          const float *p = p0 + k * step + (k == 0 ? 0 : tail);
+          ml[q] = __ldcg(reinterpret_cast<const float2 *>(p - kPer * lane + D));
+          if constexpr (kPer == 4) *reinterpret_cast<float4 *>(x[q]) = __ldcg(reinterpret_cast<const float4 *>(p));
+          else *reinterpret_cast<float2 *>(x[q]) = __ldcg(reinterpret_cast<const float2 *>(p));
+          if (k0 + q * share >= np) ml[q] = make_float2(-INFINITY, 0.f);
+        }
+        float mn = M;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) mn = fmaxf(mn, ml[q].x);
+        const float ref = mn == -INFINITY ? 0.f : mn, corr = fast_exp2(M - ref);
+        M = mn;
+        L *= corr;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) y[e] *= corr;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          if (k0 + q * share >= np) continue;
+          const float w = fast_exp2(ml[q].x - ref);  // (0 times a NaN state: NaN)
+          L = fmaf(w, ml[q].y, L);
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) y[e] = fmaf(w, x[q][e], y[e]);
+        }
       }
-      L += warp_sum(lw);
-      const int n = min(32, np - k0);
-#pragma unroll 8
-      for (int k = 0; k < n; ++k) {
-        const float wk = __shfl_sync(0xffffffffu, w, k);
-        const float *p = at(k0 + k);
+      if (share > 1) {
+        __syncthreads();  // the last row's sums have been read
+        if (lane == 0) {
+          s_ml[warp][0] = M;
+          s_ml[warp][1] = L;
+        }
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) y[e] += wk * p[32 * e + lane];
+        for (int e = 0; e < kPer; ++e) s_o[warp][kPer * lane + e] = y[e];
+        __syncthreads();
+        if (live && first == 0) {
+          float mn = M;
+          for (int w = 1; w < share; ++w) mn = fmaxf(mn, s_ml[warp + w][0]);
+          const float ref = mn == -INFINITY ? 0.f : mn, corr = fast_exp2(M - ref);
+          L *= corr;
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) y[e] *= corr;
+          for (int w = 1; w < share; ++w) {
+            const float f = fast_exp2(s_ml[warp + w][0] - ref);
+            L = fmaf(f, s_ml[warp + w][1], L);
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) y[e] = fmaf(f, s_o[warp + w][kPer * lane + e], y[e]);
+          }
+        }
+      }
+      if (live && first == 0) {
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        T *o = static_cast<T *>(out) + (size_t)(row0 + i) * (size_t)o_row + (size_t)(head0 + j) * (size_t)o_head;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) o[kPer * lane + e] = from_float<T>(y[e] * inv);
       }
     }
-    const float inv = M == -INFINITY ? 0.f : 1.f / L;
-    T *o = static_cast<T *>(out) + (size_t)(row0 + i) * (size_t)o_row + (size_t)(head0 + j) * (size_t)o_head;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) o[32 * e + lane] = from_float<T>(y[e] * inv);
   }
 }
 
 // ---------------------------------------------------------------- host side
 constexpr int kMaxDevices = 64;
 constexpr int kMaxSms = 160;
-constexpr int kMaxCtas = 3 * kMaxSms;
-constexpr size_t kDescBytes = ((size_t)kMaxCtas * 2 * kDescWords * 4 + 255) / 256 * 256;
+constexpr int kMaxWorkers = 12 * kMaxSms;
+constexpr size_t kDescBytes = ((size_t)kMaxWorkers * kDescWords * 4 + 255) / 256 * 256;
 
 std::mutex g_mutex;
 
-int encode_codes(CUtensorMap *m, const QmkKvCache *c, void *codes, int tile) {
+int encode_codes(CUtensorMap *m, const QmkKvCache *c, void *codes) {
   static PFN_cuTensorMapEncodeTiled_v12000 enc = nullptr;
   {
     std::lock_guard<std::mutex> lock(g_mutex);
@@ -842,16 +856,14 @@ int encode_codes(CUtensorMap *m, const QmkKvCache *c, void *codes, int tile) {
       enc = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
     }
   }
+  // rows of 32, 64 or 128 bytes as lines of 128, boxes of one tile (Shape::kTile)
   const cuuint64_t row = (cuuint64_t)c->head_dim * c->bits / 8, head = row * c->capacity;
   const cuuint64_t seq = c->num_seqs > 1 ? (cuuint64_t)c->code_seq_stride : head * c->num_kv_heads;
-  const cuuint64_t dims[4] = {row, (cuuint64_t)c->capacity, (cuuint64_t)c->num_kv_heads, (cuuint64_t)c->num_seqs};
-  const cuuint64_t strides[3] = {row, head, seq};
-  const cuuint32_t box[4] = {(cuuint32_t)row, (cuuint32_t)tile, 1, 1}, one[4] = {1, 1, 1, 1};
-  const CUtensorMapSwizzle sw = row == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
-                                : row == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
-                                            : CU_TENSOR_MAP_SWIZZLE_32B;
+  const cuuint64_t dims[4] = {128, head / 128, (cuuint64_t)c->num_kv_heads, (cuuint64_t)c->num_seqs};
+  const cuuint64_t strides[3] = {128, head, seq};
+  const cuuint32_t box[4] = {128, (cuuint32_t)(row == 128 ? 32 : row / 2), 1, 1}, one[4] = {1, 1, 1, 1};
   const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, codes, dims, strides, box, one,
-                         CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(QMK_ERR_ARGS, "cuTensorMapEncodeTiled rejected the cache");
   return QMK_OK;
@@ -894,7 +906,7 @@ int check_attend(const char *who, const QmkKvCache *c, const QmkKvRows *r, int n
 
 size_t workspace_need(const QmkKvCache *c, const QmkKvRows *r, int num_q_heads, int dtype) {
   const int slots = slots_of(dtype, tiles_n(dtype, r->max_rows, num_q_heads / c->num_kv_heads));
-  const size_t parts = (size_t)kMaxCtas * 2 * slots * (c->head_dim + 2) * 4;
+  const size_t parts = (size_t)kMaxWorkers * 2 * slots * (c->head_dim + 4) * 4;
   return kDescBytes + (parts + 255) / 256 * 256;
 }
 
@@ -911,13 +923,14 @@ int launch_attend(AttendArgs &a, int sms, int dev, cudaStream_t stream) {
       ready[dev] = true;
     }
   }
-  const int grid = std::min(sms * S::kCtas, kMaxCtas);
+  const int grid = std::min(sms, kMaxSms);
   int rb, hb, head_blocks;
   block_shape(S::kSlots, a.ratio, rb, hb, head_blocks);
-  cudaError_t e = launch_pdl(attend_kernel<T, BITS, D, NT>, grid, 32 * kWarps, S::kSmem, stream, a);
+  cudaError_t e = launch_pdl(attend_kernel<T, BITS, D, NT>, grid, 32 * S::kWarps, S::kSmem, stream, a);
   if (e == cudaSuccess)
-    e = launch_pdl(merge_kernel<T, D>, grid, 128, 0, stream, (const int *)a.desc, (const float *)a.parts,
-                   (int)S::kSlots, hb, a.out, a.o_row, a.o_head);
+    e = launch_pdl(merge_kernel<T, D>, std::min(grid * S::kWarps, 4 * sms), 32 * kMergeWarps, 0, stream,
+                   (const int *)a.desc, (const float *)a.parts, grid * S::kWarps, (int)S::kSlots, hb, a.out, a.o_row,
+                   a.o_head);
   if (e != cudaSuccess) return fail(QMK_ERR_CUDA, "qmk_kv_attend launch: %s", cudaGetErrorString(e));
   return QMK_OK;
 }
@@ -965,8 +978,8 @@ extern "C" int qmk_kv_attend(const QmkKvCache *cache, const QmkKvRows *rows, con
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return fail(QMK_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
   AttendArgs a;
-  rc = encode_codes(&a.k_map, cache, cache->k_codes, kTile);
-  if (rc == QMK_OK) rc = encode_codes(&a.v_map, cache, cache->v_codes, kTile);
+  rc = encode_codes(&a.k_map, cache, cache->k_codes);
+  if (rc == QMK_OK) rc = encode_codes(&a.v_map, cache, cache->v_codes);
   if (rc != QMK_OK) return rc;
   a.k_scales = static_cast<const __nv_bfloat16 *>(cache->k_scales);
   a.v_scales = static_cast<const __nv_bfloat16 *>(cache->v_scales);
