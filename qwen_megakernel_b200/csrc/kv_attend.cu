@@ -463,6 +463,8 @@ __global__ void __launch_bounds__(32 * Shape<T, BITS, D, NT>::kWarps, 1)
         lim[t][i] = slot_limit(SPLIT ? 4 * t + tig : 8 * t + 2 * tig + i);
       }
     }
+    // positions below this are seen by every row of the block
+    const int seen_by_all = ok_rows == nrows ? len - ok_rows + 1 : 0;
     float m[NT][NS], l[NT][NS];
     float acc[NT][G][2][4];
 #pragma unroll
@@ -521,8 +523,7 @@ __global__ void __launch_bounds__(32 * Shape<T, BITS, D, NT>::kWarps, 1)
 #pragma unroll
           for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int k = 0; k < 4; ++k)  // what the slot's row does not see starts from -inf
-              s[t][k] = pos0 + p0 + 16 * sub + 8 * (k >> 1) + gid < lim[t][SPLIT ? 0 : (k & 1)] ? 0.f : -INFINITY;
+            for (int k = 0; k < 4; ++k) s[t][k] = 0.f;
 #pragma unroll
           for (int c2 = 0; c2 < S::kChunks; c2 += 2) {
             unsigned w[4];  // chunk c2: rows gid, gid + 8; chunk c2 + 1: the same
@@ -569,6 +570,17 @@ __global__ void __launch_bounds__(32 * Shape<T, BITS, D, NT>::kWarps, 1)
                 x[sub][t][r][1] = s[t][2 * r + 1];
               }
             }
+        }
+        if (pos0 + p0 + 32 > seen_by_all) {
+#pragma unroll
+          for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int k = 0; k < NS; ++k)
+                  if (pos0 + p0 + 16 * sub + 8 * r + gid >= lim[t][k]) x[sub][t][r][k] = -INFINITY;
         }
         // V scales of this lane's positions, and the exponent of the largest
         uint2 vw[2][2];

@@ -1,11 +1,14 @@
 // Quantized K/V cache: rows quantized as they are written, and read back
 // (qmk_kv_write, qmk_kv_read; the format is in include/qwen_megakernel.h).
 //
-// Both are one pass over the data: a thread owns 8 consecutive dimensions of
-// one row and head (16 bytes of bf16, one 32-bit word of 4-bit codes), 4
-// neighbouring lanes one group of 32, so the group's largest magnitude is two
-// shuffles and every access is a full, coalesced vector.
+// Both are one pass over the data, bound by the row tensors' bytes (bf16: 256
+// of a row and head's 328).  A thread owns 8 consecutive dimensions of one
+// head (16 bytes of bf16, one 32-bit word of 4-bit codes) in a few rows, K and
+// V alike, with all its loads issued first; 4 neighbouring lanes hold a group
+// of 32, so the group's largest magnitude is two shuffles.  A CTA looks its
+// rows' sequences and positions up once, in shared memory.
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 
@@ -86,7 +89,6 @@ struct Side {
   __nv_bfloat16 *scales;
   T *x;
   long long row_stride, head_stride;
-  bool aligned;
 };
 
 template <typename T>
@@ -94,122 +96,267 @@ struct Args {
   Side<T> side[2];  // K, V
   Rows rows;
   long long code_seq_stride, scale_seq_stride;
-  int heads, capacity;
+  int heads, capacity, rows_per_cta;
   unsigned *status;
 };
 
 constexpr int kThreads = 256;
+constexpr int kMaxRowsPerCta = 64;
+constexpr int kBatch = 2;  // rows of a thread in flight
 
-// rint(x / s) for |x| <= s * (127 + 1/2), s a normal bf16: exact, with one
-// reciprocal for the group.  r = rint(x * (1 / s)) can miss only at a
-// border between two codes; d = x - r s has no rounding error (r s has at
-// most 15 significant bits; for r != 0 x and r s are within a factor 2 of
-// each other), so the comparison of |d| with s / 2 decides, ties to even.
-__device__ __forceinline__ float code_of(float x, float s, float inv, float half) {
-  float r = rintf(x * inv);
-  const float d = fmaf(-r, s, x), ad = fabsf(d);
-  if (ad > half || (ad == half && (static_cast<int>(r) & 1))) r += copysignf(1.f, d);
-  return r;
-}
+// Where the CTA's rows lie, looked up once: offsets of their sequence and
+// position (the head's come on top), -1 where no segment holds the row, -2
+// where it is out of range.
+struct RowTable {
+  long long code[kMaxRowsPerCta];
+  long long scale[kMaxRowsPerCta];
+};
 
 template <typename T, int BITS, int D>
+__device__ __forceinline__ int fill_rows(RowTable &t, const Args<T> &a, int row0) {
+  const int n = min(a.rows_per_cta, a.rows.rows - row0);
+  if ((int)threadIdx.x < n) {
+    int seq = 0, pos = 0;
+    const int ok = locate_row(a.rows, row0 + threadIdx.x, seq, pos);
+    if (ok < 0 && a.status) atomicOr(a.status, QMK_KV_BAD_ROW);
+    t.code[threadIdx.x] = ok > 0 ? seq * a.code_seq_stride + (long long)pos * (D * BITS / 8) : ok - 1;
+    t.scale[threadIdx.x] = seq * a.scale_seq_stride + (long long)pos * (D / kGroup);
+  }
+  __syncthreads();
+  return n;
+}
+
+__device__ __forceinline__ float fast_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// x / s, correctly rounded for what is asked here, from r ~ 1 / s: one Newton
+// step on the quotient with its exact remainder (Markstein's division).  Its
+// error before the last rounding is below 2^-44 of the quotient, so a quotient
+// that fp32 holds (the border of two codes, or of two bf16 scales, among them)
+// comes out exactly, and one that lies off a border is not rounded onto it: x
+// and s have 24 and 8 bits, the nearest such quotient is more than half a step
+// of fp32 away.  Both within 2^-100 .. 2^126.
+__device__ __forceinline__ float divide(float x, float s, float r) {
+  const float q = x * r;
+  return fmaf(fmaf(-q, s, x), r, q);
+}
+
+// 8 values of a group to codes, words packed; any scale, any value.
+template <int BITS>
+__device__ __forceinline__ void codes_any(const float (&x)[8], float s, unsigned (&word)[BITS / 4]) {
+  constexpr float kTop = BITS == 4 ? 7.f : 127.f, kOffset = BITS == 4 ? 8.f : 128.f;
+#pragma unroll
+  for (int i = 0; i < BITS / 4; ++i) word[i] = 0u;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float c = 0.f;
+    if (s != 0.f && x[i] == x[i]) c = fminf(fmaxf(rintf(__fdiv_rn(x[i], s)), -kTop), kTop);
+    word[i * BITS / 32] |= (unsigned)(int)(c + kOffset) << (i * BITS % 32);
+  }
+}
+
+// Codes and scale of a thread's 8 values; the 4 lanes of a group agree.
+template <int BITS>
+__device__ __forceinline__ __nv_bfloat16 quantize8(const float (&x)[8], unsigned (&word)[BITS / 4], unsigned *status) {
+  constexpr float kTop = BITS == 4 ? 7.f : 127.f;
+  unsigned top = 0;  // bits of the largest magnitude, infinities and NaN above all
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+  // largest magnitude within 2^-90 .. 2^126: scale and quotients are ordinary numbers
+  const bool easy = top >= 0x12800000u && top < 0x7e800000u;
+  if (__all_sync(0xffffffffu, easy)) {
+    const __nv_bfloat16 sb = __float2bfloat16_rn(divide(__uint_as_float(top), kTop, 1.f / kTop));
+    const float s = __bfloat162float(sb), r = fast_rcp(s);
+    // x / s + 1.5 2^23 + offset holds the code, rounded to even, in its low
+    // bits; in a word's sum the patterns above the codes add up to a constant
+    constexpr float kMagic = 12582912.f + (BITS == 4 ? 8.f : 128.f);
+    constexpr int kPer = 32 / BITS;
+    unsigned above = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) above += 0x4b400000u << (BITS * i);
+#pragma unroll
+    for (int w = 0; w < BITS / 4; ++w) {
+      unsigned sum = 0u - above;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        sum += __float_as_uint(divide(x[kPer * w + i], s, r) + kMagic) * (1u << (BITS * i));
+      word[w] = sum;
+    }
+    return sb;
+  }
+  unsigned fin = 0;  // largest finite magnitude
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const unsigned u = __float_as_uint(x[i]) & 0x7fffffffu;
+    fin = max(fin, u < 0x7f800000u ? u : 0u);
+  }
+  fin = max(fin, __shfl_xor_sync(0xffffffffu, fin, 1));
+  fin = max(fin, __shfl_xor_sync(0xffffffffu, fin, 2));
+  if (top >= 0x7f800000u && status) atomicOr(status, QMK_KV_NONFINITE);
+  const __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(__uint_as_float(fin), kTop));
+  codes_any<BITS>(x, __bfloat162float(sb), word);
+  return sb;
+}
+
+// 8 elements as they lie in memory; single loads unless VEC.
+template <typename T, bool VEC>
+struct Raw {
+  uint4 w[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T *p) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) reinterpret_cast<T *>(w)[i] = p[i];
+    }
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_float(reinterpret_cast<const T *>(w)[i]);
+  }
+};
+
+template <typename T, int BITS, int D, bool VEC>
 __global__ void __launch_bounds__(kThreads) write_kernel(const __grid_constant__ Args<T> a) {
+  __shared__ RowTable tab;
   qmk::pdl_wait();  // rows and cache may be touched by the previous kernel
   qmk::pdl_trigger();
   constexpr int kChunks = D / 8;
-  constexpr float kTop = BITS == 4 ? 7.f : 127.f;
-  const Side<T> &sd = a.side[blockIdx.y];
-  const long long unit = ((long long)blockIdx.x * kThreads + threadIdx.x) / kChunks;  // (row, head)
-  const int chunk = threadIdx.x % kChunks;
-  const long long row = unit / a.heads;
-  const int head = (int)(unit - row * a.heads);
-  int seq = 0, pos = 0, ok = 0;
-  if (row < a.rows.rows) ok = locate_row(a.rows, (int)row, seq, pos);
-  if (ok < 0 && chunk == 0 && head == 0 && a.status) atomicOr(a.status, QMK_KV_BAD_ROW);
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (ok > 0)
-    load_n<T, 8>(sd.x + (size_t)row * (size_t)sd.row_stride + (size_t)head * (size_t)sd.head_stride + 8 * chunk,
-                 sd.aligned, x);
-  float top = 0.f;
-  bool odd = false;
+  const int row0 = blockIdx.x * a.rows_per_cta;
+  const int n = fill_rows<T, BITS, D>(tab, a, row0);
+  const int cols = a.heads * kChunks;                               // (head, chunk) pairs, a multiple of 8
+  const int width = min(cols, kThreads), lines = kThreads / width;  // threads a row, rows at once
+  const int line = threadIdx.x / width;
+  // (all lanes of a warp run the same trips, for the shuffles: those without a value idle along)
+  for (int base = 0; base < cols; base += width) {
+    const int c0 = base + threadIdx.x - line * width;
+    const int head = c0 / kChunks, chunk = c0 % kChunks;
+    const bool in = line < lines && c0 < cols;
+    const T *src[2];
+    uint8_t *codes[2];
+    __nv_bfloat16 *scales[2];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float m = fabsf(x[i]);
-    const bool fin = m < INFINITY;  // false for NaN too
-    odd |= !fin;
-    top = fin ? fmaxf(top, m) : top;
-  }
-  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-  top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-  if (odd && a.status) atomicOr(a.status, QMK_KV_NONFINITE);
-  if (ok <= 0) return;
-  const __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(top, kTop));
-  const float s = __bfloat162float(sb);
-  unsigned word[BITS / 4] = {};
-  constexpr float kOffset = BITS == 4 ? 8.f : 128.f;
-  // The reciprocal needs s well inside the normal range (2^-100 .. 2^126).
-  const bool normal = s > 7.9e-31f && s < 8e37f;
-  const float inv = __frcp_rn(s), half = 0.5f * s;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float c;
-    if (s == 0.f) {
-      c = 0.f;
-    } else if (!(fabsf(x[i]) < INFINITY)) {
-      c = (x[i] != x[i]) ? 0.f : copysignf(kTop, x[i]);
-    } else {
-      c = normal ? code_of(x[i], s, inv, half) : rintf(__fdiv_rn(x[i], s));
-      c = fminf(fmaxf(c, -kTop), kTop);  // beyond only where s is rounded coarsely (subnormal)
+    for (int i = 0; i < 2; ++i) {
+      const Side<T> &sd = a.side[i];
+      src[i] = sd.x + (size_t)row0 * (size_t)sd.row_stride + (size_t)head * (size_t)sd.head_stride + 8 * chunk;
+      codes[i] = sd.codes + (size_t)head * (size_t)a.capacity * (D * BITS / 8) + BITS * chunk;
+      scales[i] = sd.scales + (size_t)head * (size_t)a.capacity * (D / kGroup) + (chunk >> 2);
     }
-    const unsigned u = (unsigned)(int)(c + kOffset);
-    word[i * BITS / 32] |= u << (i * BITS % 32);
+    for (int r0 = 0; r0 < n; r0 += kBatch * lines) {
+      Raw<T, VEC> raw[kBatch][2];
+      bool ok[kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int r = r0 + k * lines + line;
+        ok[k] = in && r < n && tab.code[r] >= 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          raw[k][i].zero();
+          if (ok[k]) raw[k][i].load(src[i] + (size_t)r * (size_t)a.side[i].row_stride);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float x[8];
+          unsigned word[BITS / 4];
+          raw[k][i].get(x);
+          const __nv_bfloat16 sb = quantize8<BITS>(x, word, a.status);
+          if (ok[k]) {
+            const int r = r0 + k * lines + line;
+            uint8_t *dst = codes[i] + tab.code[r];
+            if constexpr (BITS == 4) *reinterpret_cast<unsigned *>(dst) = word[0];
+            else *reinterpret_cast<uint2 *>(dst) = make_uint2(word[0], word[1]);
+            if ((chunk & 3) == 0) scales[i][tab.scale[r]] = sb;
+          }
+        }
+    }
   }
-  const size_t at = (size_t)head * (size_t)a.capacity + (size_t)pos;
-  uint8_t *dst = sd.codes + (size_t)seq * (size_t)a.code_seq_stride + at * (D * BITS / 8) + chunk * BITS;
-  if constexpr (BITS == 4) *reinterpret_cast<unsigned *>(dst) = word[0];
-  else *reinterpret_cast<uint2 *>(dst) = make_uint2(word[0], word[1]);
-  if ((chunk & 3) == 0)
-    sd.scales[(size_t)seq * (size_t)a.scale_seq_stride + at * (D / kGroup) + (chunk >> 2)] = sb;
 }
 
-template <typename T, int BITS, int D>
+template <typename T, int BITS, int D, bool VEC>
 __global__ void __launch_bounds__(kThreads) read_kernel(const __grid_constant__ Args<T> a) {
+  __shared__ RowTable tab;
   qmk::pdl_wait();  // the cache is written by the previous kernel
   qmk::pdl_trigger();
   constexpr int kChunks = D / 8;
-  const Side<T> &sd = a.side[blockIdx.y];
-  const long long unit = ((long long)blockIdx.x * kThreads + threadIdx.x) / kChunks;
-  const int chunk = threadIdx.x % kChunks;
-  const long long row = unit / a.heads;
-  const int head = (int)(unit - row * a.heads);
-  if (row >= a.rows.rows) return;
-  int seq = 0, pos = 0;
-  const int ok = locate_row(a.rows, (int)row, seq, pos);
-  if (ok == 0) return;
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (ok > 0) {
-    const size_t at = (size_t)head * (size_t)a.capacity + (size_t)pos;
-    const uint8_t *src = sd.codes + (size_t)seq * (size_t)a.code_seq_stride + at * (D * BITS / 8) + chunk * BITS;
-    const float s =
-        __bfloat162float(sd.scales[(size_t)seq * (size_t)a.scale_seq_stride + at * (D / kGroup) + (chunk >> 2)]);
-    unsigned word[BITS / 4];
-    if constexpr (BITS == 4) {
-      word[0] = *reinterpret_cast<const unsigned *>(src);
-    } else {
-      const uint2 w = *reinterpret_cast<const uint2 *>(src);
-      word[0] = w.x;
-      word[1] = w.y;
-    }
+  const int row0 = blockIdx.x * a.rows_per_cta;
+  const int n = fill_rows<T, BITS, D>(tab, a, row0);
+  const int cols = a.heads * kChunks;
+  const int width = min(cols, kThreads), lines = kThreads / width;
+  const int line = threadIdx.x / width;
+  if (line >= lines) return;
+  for (int c0 = threadIdx.x - line * width; c0 < cols; c0 += width) {
+    const int head = c0 / kChunks, chunk = c0 % kChunks;
+    const uint8_t *codes[2];
+    const __nv_bfloat16 *scales[2];
+    T *dst[2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int u = (int)((word[i * BITS / 32] >> (i * BITS % 32)) & ((1u << BITS) - 1u));
-      x[i] = s * (float)(u - (1 << (BITS - 1)));
+    for (int i = 0; i < 2; ++i) {
+      const Side<T> &sd = a.side[i];
+      dst[i] = sd.x + (size_t)row0 * (size_t)sd.row_stride + (size_t)head * (size_t)sd.head_stride + 8 * chunk;
+      codes[i] = sd.codes + (size_t)head * (size_t)a.capacity * (D * BITS / 8) + BITS * chunk;
+      scales[i] = sd.scales + (size_t)head * (size_t)a.capacity * (D / kGroup) + (chunk >> 2);
     }
-  } else if (chunk == 0 && head == 0 && a.status) {
-    atomicOr(a.status, QMK_KV_BAD_ROW);
+    for (int r0 = line; r0 < n; r0 += kBatch * lines) {
+      unsigned word[kBatch][2][BITS / 4];
+      float s[kBatch][2];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int r = r0 + k * lines;
+        const bool ok = r < n && tab.code[r] >= 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          // a row out of range reads as zeros: the scale is 0
+          s[k][i] = 0.f;
+#pragma unroll
+          for (int e = 0; e < BITS / 4; ++e) word[k][i][e] = 0u;
+          if (ok) {
+            s[k][i] = __bfloat162float(scales[i][tab.scale[r]]);
+            if constexpr (BITS == 4) {
+              word[k][i][0] = *reinterpret_cast<const unsigned *>(codes[i] + tab.code[r]);
+            } else {
+              const uint2 w = *reinterpret_cast<const uint2 *>(codes[i] + tab.code[r]);
+              word[k][i][0] = w.x;
+              word[k][i][1] = w.y;
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int r = r0 + k * lines;
+        if (r >= n || tab.code[r] == -1) continue;  // (-1: no segment holds the row)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int u = (int)((word[k][i][e * BITS / 32] >> (e * BITS % 32)) & ((1u << BITS) - 1u));
+            x[e] = s[k][i] * (float)(u - (1 << (BITS - 1)));  // exact: 8 + 7 significant bits
+          }
+          store_n<T, 8>(dst[i] + (size_t)r * (size_t)a.side[i].row_stride, VEC, x);
+        }
+      }
+    }
   }
-  store_n<T, 8>(sd.x + (size_t)row * (size_t)sd.row_stride + (size_t)head * (size_t)sd.head_stride + 8 * chunk,
-                sd.aligned, x);
+}
+
+template <typename T, bool WRITE, int BITS, int D>
+void (*pick(bool vec))(const Args<T>) {
+  if constexpr (WRITE) return vec ? write_kernel<T, BITS, D, true> : write_kernel<T, BITS, D, false>;
+  else return vec ? read_kernel<T, BITS, D, true> : read_kernel<T, BITS, D, false>;
 }
 
 template <typename T, bool WRITE>
@@ -220,26 +367,26 @@ int launch(const QmkKvCache *c, const QmkKvRows *r, const QmkKvTensor *k, const 
   void *codes[2] = {c->k_codes, c->v_codes}, *scales[2] = {c->k_scales, c->v_scales};
   for (int i = 0; i < 2; ++i)
     a.side[i] = Side<T>{static_cast<uint8_t *>(codes[i]), static_cast<__nv_bfloat16 *>(scales[i]),
-                        static_cast<T *>(t[i]->data), t[i]->row_stride, t[i]->head_stride, vector_aligned(t[i])};
+                        static_cast<T *>(t[i]->data), t[i]->row_stride, t[i]->head_stride};
   a.rows = device_rows(c, r);
   a.code_seq_stride = c->code_seq_stride;
   a.scale_seq_stride = c->scale_seq_stride;
   a.heads = c->num_kv_heads;
   a.capacity = c->capacity;
   a.status = status;
-  const long long threads = (long long)r->rows * c->num_kv_heads * (c->head_dim / 8);
-  const long long blocks = (threads + kThreads - 1) / kThreads;
-  if (blocks > 0x7fffffffLL) return fail(QMK_ERR_ARGS, "qmk_kv: too many rows");
-  void (*kernel)(const Args<T>) = nullptr;
-  if (c->head_dim == 128) {
-    if (c->bits == 4) kernel = WRITE ? write_kernel<T, 4, 128> : read_kernel<T, 4, 128>;
-    else kernel = WRITE ? write_kernel<T, 8, 128> : read_kernel<T, 8, 128>;
-  } else {
-    if (c->bits == 4) kernel = WRITE ? write_kernel<T, 4, 64> : read_kernel<T, 4, 64>;
-    else kernel = WRITE ? write_kernel<T, 8, 64> : read_kernel<T, 8, 64>;
-  }
+  // rows a CTA: enough for its threads' batches, fewer while that leaves SMs without work
+  const int width = std::min(c->num_kv_heads * (c->head_dim / 8), kThreads);
+  const int batch = kBatch * (kThreads / width);
+  int per = std::min(kMaxRowsPerCta, 4 * batch);
+  while (per > 1 && (r->rows + per - 1) / per < 4 * 148) per = (per + 1) / 2;
+  a.rows_per_cta = per;
+  const int blocks = (r->rows + per - 1) / per;
+  const bool vec = vector_aligned(k) && vector_aligned(v);
+  void (*kernel)(const Args<T>) =
+      c->head_dim == 128 ? (c->bits == 4 ? pick<T, WRITE, 4, 128>(vec) : pick<T, WRITE, 8, 128>(vec))
+                         : (c->bits == 4 ? pick<T, WRITE, 4, 64>(vec) : pick<T, WRITE, 8, 64>(vec));
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)blocks, 2);
+  cfg.gridDim = dim3((unsigned)blocks);
   cfg.blockDim = dim3(kThreads);
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
