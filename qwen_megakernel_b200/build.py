@@ -49,11 +49,13 @@ KERNEL_SOURCES = [
     os.path.join(CSRC, "gemm_tc.cu"),
     os.path.join(CSRC, "kv_cache.cu"),
     os.path.join(CSRC, "kv_attend.cu"),
+    os.path.join(CSRC, "kv_attend_tc.cu"),
 ]
 KERNEL_DEPS = KERNEL_SOURCES + [
     os.path.join(CSRC, "qmk_device.cuh"),
     os.path.join(CSRC, "qmk_schedule.h"),
     os.path.join(CSRC, "kv_cache.cuh"),
+    os.path.join(CSRC, "kv_attend.cuh"),
     os.path.join(INCLUDE, "qwen_megakernel.h"),
 ]
 OPS_SOURCES = [os.path.join(CSRC, "torch_bindings.cpp")]

@@ -21,107 +21,20 @@
 // pair hi + lo on two columns of the same product, as is p s (2^-22).
 // Scores, maxima, sums and outputs are fp32.
 
-#include <cuda.h>
 #include <cudaTypedefs.h>
 
 #include <algorithm>
 #include <mutex>
 
-#include "kv_cache.cuh"
+#include "kv_attend.cuh"
 
 int qmk_internal_set_error(int code, const char *msg);
 int qmk_internal_clear_error();
 
 namespace qkv {
 
-using namespace qmk;
-
-constexpr unsigned long long kWaitNs = 1000000000ull;  // bound on one copy wait
 constexpr float kLog2e = 1.4426950408889634f;
 
-struct AttendArgs {
-  CUtensorMap k_map, v_map;  // codes: dims {128 bytes, 128-byte lines, heads, sequences}
-  const __nv_bfloat16 *k_scales, *v_scales;
-  long long scale_seq_stride;
-  int capacity, heads, ratio;
-  Rows rows;
-  const void *q;
-  void *out;
-  long long q_row, q_head, o_row, o_head;
-  bool q_aligned;
-  float scale_log2;  // softmax scale * log2(e)
-  int *desc;         // workspace: per worker a descriptor of kDescWords
-  float *parts;      // workspace: per worker 2 x slots x (D + 4)
-  unsigned *status;
-};
-
-// ------------------------------------------------------------- work division
-// The query rows of one segment and K/V head are cut into blocks of rb rows
-// by hb of the K/V head's q heads; a block and its positions [0, len), in
-// tiles, are an item.  All items' tiles in order (segment, K/V head, head
-// block, row block) form one list that is dealt to the workers (warps) in
-// equal contiguous ranges, so ragged lengths, few items and many all load
-// every SM alike; an item cut by a range border leaves parts that
-// merge_kernel joins, in order.
-struct Segment {
-  int r0, n;      // rows
-  int ok_rows;    // the first ok_rows of them are in range
-  int start, seq;
-  int blocks;     // row blocks
-  int ok_blocks;  // those that hold a row in range
-  long long units;       // tiles of one (K/V head, head block)
-};
-
-// sum of floor((a i + b) / m) over i < n, by the Euclidean exchange of a and m
-__device__ inline long long floor_sum(long long n, unsigned m, unsigned a, unsigned b) {
-  long long sum = 0;
-  unsigned k = (unsigned)n;
-  while (k > 0) {
-    if (a >= m) {
-      sum += (long long)(k - 1) * k / 2 * (a / m);
-      a %= m;
-    }
-    if (b >= m) {
-      sum += (long long)k * (b / m);
-      b %= m;
-    }
-    const unsigned long long y = (unsigned long long)a * k + b;
-    if (y < m) break;
-    const unsigned nk = (unsigned)(y / m);
-    b = (unsigned)(y % m);
-    k = nk;
-    const unsigned t = m;
-    m = a;
-    a = t;
-  }
-  return sum;
-}
-
-// Tiles of row blocks [0, cb) of a segment, cb <= s.blocks.
-template <int TILE>
-__device__ inline long long block_prefix(const Segment &s, int rb, int cb) {
-  long long u = 0;
-  const int whole = min(cb, s.ok_blocks - 1);  // the last block in range may be cut
-  if (whole > 0) u = floor_sum(whole, TILE, rb, s.start + rb + TILE - 1);
-  if (cb >= s.ok_blocks && s.ok_blocks > 0) u += (s.start + s.ok_rows + TILE - 1) / TILE;
-  return u + max(0, cb - s.ok_blocks);  // a block out of range: one empty tile
-}
-
-template <int TILE>
-__device__ inline Segment load_segment(const Rows &R, int b, int rb) {
-  Segment s;
-  segment_rows(R, b, s.r0, s.n);
-  s.seq = segment_seq(R, b);
-  s.start = R.start[b];
-  const bool ok = s.seq >= 0 && s.seq < R.num_seqs && s.start >= 0 && s.start < R.max_seq_len;
-  s.ok_rows = ok ? min(s.n, min(R.max_rows, R.max_seq_len - s.start)) : 0;
-  s.blocks = (s.n + rb - 1) / rb;
-  s.ok_blocks = (s.ok_rows + rb - 1) / rb;
-  s.units = block_prefix<TILE>(s, rb, s.blocks);
-  return s;
-}
-
-constexpr int kDescWords = 8;
 
 // ------------------------------------------------------------- instructions
 __device__ __forceinline__ void mma_f16(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
@@ -153,69 +66,6 @@ __device__ __forceinline__ unsigned transpose8(unsigned x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
-__device__ __forceinline__ unsigned max_u16x2(unsigned a, unsigned b) {
-  unsigned y;
-  asm("max.u16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
-  return y;
-}
-__device__ __forceinline__ float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ unsigned pack_f16(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const unsigned *>(&h);
-}
-__device__ __forceinline__ unsigned hadd2(unsigned x, unsigned c) {
-  unsigned y;
-  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(c));
-  return y;
-}
-__device__ __forceinline__ unsigned hfma2(unsigned x, unsigned m, unsigned c) {
-  unsigned y;
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(y) : "r"(x), "r"(m), "r"(c));
-  return y;
-}
-// Constants of the decoding, kept in registers: an instruction takes one
-// immediate operand, and these are second ones.
-struct Decode {
-  unsigned exp, off;
-  __device__ __forceinline__ explicit Decode(int bits) {
-    asm volatile("mov.b32 %0, %1;" : "=r"(exp) : "r"(bits == 4 ? 0x64006400u : 0x64646464u));
-    asm volatile("mov.b32 %0, %1;" : "=r"(off) : "r"(0xd480d480u));  // -72
-  }
-  template <unsigned MASK>
-  __device__ __forceinline__ unsigned take(unsigned w) const {  // (w & MASK) | exp
-    unsigned y;
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(y) : "r"(w), "n"(MASK), "r"(exp));
-    return y;
-  }
-  // The fp16 values u - 8 of nibbles (0, 4), (1, 5), (2, 6), (3, 7) of w.
-  __device__ __forceinline__ void nibbles(unsigned w, unsigned (&h)[4]) const {
-    const unsigned v = w >> 8;
-    h[0] = hadd2(take<0x000f000fu>(w), 0xe408e408u);        // 1024 + u - 1032
-    h[1] = hfma2(take<0x00f000f0u>(w), 0x2c002c00u, off);  // (1024 + 16 u) / 16 - 72
-    h[2] = hadd2(take<0x000f000fu>(v), 0xe408e408u);
-    h[3] = hfma2(take<0x00f000f0u>(v), 0x2c002c00u, off);
-  }
-  // The fp16 values u - 128 of bytes (0, 2) and (1, 3) of w.
-  __device__ __forceinline__ void bytes(unsigned w, unsigned (&h)[2]) const {
-    h[0] = hadd2(__byte_perm(w, exp, 0x4240), 0xe480e480u);  // 1024 + u - 1152
-    h[1] = hadd2(__byte_perm(w, exp, 0x4341), 0xe480e480u);
-  }
-};
-__device__ __forceinline__ float f16_round(float x) { return __half2float(__float2half_rn(x)); }
-
-__device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, int x, int y, int z, int w,
-                                            uint64_t *bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_addr(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_addr(bar))
-      : "memory");
-}
-
 __device__ __forceinline__ bool wait_copy(uint64_t *bar, unsigned parity) {
   uint64_t t0 = 0;
   for (unsigned it = 0;; ++it) {
@@ -259,13 +109,6 @@ struct Shape {
   static_assert(kStages >= 2 && kSmem <= 226 * 1024, "ring");
 };
 
-// Rows and q heads that share an item's slots.
-__host__ __device__ inline void block_shape(int slots, int ratio, int &rb, int &hb, int &head_blocks) {
-  hb = min(ratio, slots);
-  rb = max(1, slots / ratio);
-  head_blocks = (ratio + hb - 1) / hb;
-}
-
 template <typename T, int BITS, int D, int NT>
 __global__ void __launch_bounds__(32 * Shape<T, BITS, D, NT>::kWarps, 1)
     attend_kernel(const __grid_constant__ AttendArgs a) {
@@ -277,7 +120,6 @@ __global__ void __launch_bounds__(32 * Shape<T, BITS, D, NT>::kWarps, 1)
   constexpr int kTile = S::kTile;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ long long s_before[32 * W], s_scan[W];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
   uint8_t *ring = smem + warp * S::kStages * S::kStageBytes;
@@ -288,45 +130,16 @@ __global__ void __launch_bounds__(32 * Shape<T, BITS, D, NT>::kWarps, 1)
   }
   int rb, hb, head_blocks;
   block_shape(SL, a.ratio, rb, hb, head_blocks);
-  const int per_seg = a.heads * head_blocks;
   pdl_wait();  // cache, queries and rows may be written by the previous kernel
   pdl_trigger();
 
-  // ---- the list of tiles: thread t counts segments [t each, (t + 1) each)
-  const int each = (a.rows.segments + 32 * W - 1) / (32 * W);
-  long long mine = 0;
-  for (int b = tid * each; b < min((tid + 1) * each, a.rows.segments); ++b)
-    mine += load_segment<kTile>(a.rows, b, rb).units * per_seg;
-  long long before = mine;  // inclusive prefix over the warp's threads
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long x = __shfl_up_sync(0xffffffffu, before, o);
-    if (lane >= o) before += x;
-  }
-  if (lane == 31) s_scan[warp] = before;
-  s_before[tid] = before - mine;
-  __syncthreads();
-  long long total = 0, base = 0;  // base: tiles counted by earlier warps
-  for (int w = 0; w < W; ++w) {
-    const long long x = s_scan[w];
-    total += x;
-    if (w < warp) base += x;
-  }
-  s_before[tid] += base;
-  __syncthreads();
   // ---- this warp's range: with few tiles, one each to the first warps of all CTAs
-  const long long workers = max(1ll, min((long long)gridDim.x * W, total)), me = (long long)warp * gridDim.x + blockIdx.x;
-  const long long u0 = me < workers ? me * total / workers : 0, u1 = me < workers ? (me + 1) * total / workers : 0;
+  const long long me = (long long)warp * gridDim.x + blockIdx.x;
+  Range rg = find_range<kTile, 32 * W>(a.rows, rb, a.heads * head_blocks, (long long)gridDim.x * W, me);
   int *desc = a.desc + me * kDescWords;
   if (lane == 0) desc[0] = 0;
-  if (u0 >= u1) return;
-  int at = 0;  // the last thread whose count starts at or before u0
-  for (int i = lane; i < 32 * W; i += 32) at += s_before[i] <= u0;
-  at = __reduce_add_sync(0xffffffffu, at) - 1;
-  // (threads past the last segment start at `total`; equal starts are segments without rows)
-  int b = at * each;
-  long long seg_at = s_before[at];
-  Segment sg = load_segment<kTile>(a.rows, b, rb);
+  if (rg.u0 >= rg.u1) return;
+  Segment sg = load_segment<kTile>(a.rows, rg.b, rb);
 
   const Decode dec(BITS);
   const uint64_t pol = l2_policy_evict_first();
@@ -337,32 +150,11 @@ __global__ void __launch_bounds__(32 * Shape<T, BITS, D, NT>::kWarps, 1)
                         ((((lr % kPerLine) * S::kChunks + (lane >> 4)) ^ ((lr / kPerLine) & 7)) << 4);
   unsigned issued = 0, used = 0;  // ring positions
   bool dead = false;              // a wait ran out
-  long long u = u0;
 
-  while (u < u1 && !dead) {
-    while (u >= seg_at + sg.units * per_seg) {
-      seg_at += sg.units * per_seg;
-      sg = load_segment<kTile>(a.rows, ++b, rb);
-    }
-    // ---- item: K/V head h, q heads from head0, row block cb, tiles [t_lo, t_hi) of `tiles`
-    const long long in_seg = u - seg_at;
-    const int hh = (int)(in_seg / sg.units), h = hh / head_blocks, head0 = (hh - h * head_blocks) * hb;
-    const long long in_head = in_seg - (long long)hh * sg.units;
-    int cb = 0;
-    for (int hi = sg.blocks; hi - cb > 1;) {
-      const int mid = (cb + hi) >> 1;
-      if (block_prefix<kTile>(sg, rb, mid) <= in_head) cb = mid;
-      else hi = mid;
-    }
-    const int row0 = cb * rb;
-    const int ok_rows = max(0, min(rb, sg.ok_rows - row0));  // rows of this block in range
-    const int nrows = min(rb, sg.n - row0);
-    const int len = ok_rows > 0 ? sg.start + row0 + ok_rows : 0;
-    const int tiles = max(1, (len + kTile - 1) / kTile);
-    const long long item_u0 = seg_at + (long long)hh * sg.units + block_prefix<kTile>(sg, rb, cb);
-    const int t_lo = (int)(u - item_u0), t_hi = (int)min((long long)tiles, u1 - item_u0);
-    u = item_u0 + t_hi;
-    const int nt = len > 0 ? t_hi - t_lo : 0;  // tiles to read
+  while (rg.u0 < rg.u1 && !dead) {
+    const Item it = next_item<kTile>(a.rows, rg, sg, rb, hb, head_blocks, a.heads);
+    const int h = it.h, head0 = it.head0, row0 = it.row0, nrows = it.nrows, ok_rows = it.ok_rows, len = it.len;
+    const int t_lo = it.t_lo, nt = len > 0 ? it.t_hi - t_lo : 0;  // tiles to read
     const size_t sc_at =
         (size_t)(len ? sg.seq : 0) * (size_t)a.scale_seq_stride + (size_t)h * (size_t)a.capacity * G;
     auto issue = [&](int i) {  // the i-th tile of the item (lane 0)
@@ -463,8 +255,7 @@ __global__ void __launch_bounds__(32 * Shape<T, BITS, D, NT>::kWarps, 1)
         lim[t][i] = slot_limit(SPLIT ? 4 * t + tig : 8 * t + 2 * tig + i);
       }
     }
-    // positions below this are seen by every row of the block
-    const int seen_by_all = ok_rows == nrows ? len - ok_rows + 1 : 0;
+    const int seen_by_all = it.seen_by_all();
     float m[NT][NS], l[NT][NS];
     float acc[NT][G][2][4];
 #pragma unroll
@@ -699,16 +490,9 @@ __global__ void __launch_bounds__(32 * Shape<T, BITS, D, NT>::kWarps, 1)
     }
 
     // ---- the item's rows, or the part of them that this range holds
-    const bool whole = t_lo == 0 && t_hi == tiles, head_part = t_lo == 0;
+    const bool whole = it.whole(), head_part = t_lo == 0;
     if (lane == 0) {
-      if (!whole && head_part) {
-        desc[1] = sg.r0 + row0;
-        desc[2] = nrows;
-        desc[3] = h * a.ratio + head0;
-        desc[4] = min(hb, a.ratio - head0);
-        // parts: this worker's and those up to the worker with the item's last tile
-        desc[0] = (int)(((item_u0 + tiles) * workers - 1) / total - me) + 1;
-      }
+      if (!whole && head_part) describe_cut(desc, it, sg, rg, me, a.ratio, hb);
       if (ok_rows < nrows && a.status) atomicOr(a.status, QMK_KV_BAD_ROW);
     }
     float *part = a.parts + (size_t)(me * 2 + (head_part ? 0 : 1)) * SL * (D + 4);
@@ -754,7 +538,7 @@ __global__ void __launch_bounds__(32 * Shape<T, BITS, D, NT>::kWarps, 1)
 // Joins the parts of items that were cut: CTA c takes the items whose first
 // tile is in the range of worker c, c + grid, ... and that go on in the next
 // ranges.  A warp takes an output row, or several share one (few rows mean
-// many parts); 8 parts are loaded at a time.
+// many parts); 8 parts are loaded at a time.  Grid y shares an item's rows.
 constexpr int kMergeWarps = 8;
 
 template <typename T, int D>
@@ -774,7 +558,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const int *__re
     if (np == 0) continue;
     const int row0 = dd[1], nrows = dd[2], head0 = dd[3], nheads = dd[4], n = nrows * nheads;
     const int share = n >= kMergeWarps ? 1 : kMergeWarps / n, at_once = kMergeWarps / share;  // warps a row, rows
-    for (int v0 = 0; v0 < n; v0 += at_once) {
+    for (int v0 = blockIdx.y * at_once; v0 < n; v0 += gridDim.y * at_once) {
       const int v = v0 + warp / share, first = warp % share;
       const bool live = v < n && warp < share * at_once;
       const int i = live ? v / nheads : 0, j = live ? v % nheads : 0;
@@ -855,7 +639,7 @@ constexpr size_t kDescBytes = ((size_t)kMaxWorkers * kDescWords * 4 + 255) / 256
 
 std::mutex g_mutex;
 
-int encode_codes(CUtensorMap *m, const QmkKvCache *c, void *codes) {
+int encode_codes(CUtensorMap *m, const QmkKvCache *c, void *codes, int tile) {
   static PFN_cuTensorMapEncodeTiled_v12000 enc = nullptr;
   {
     std::lock_guard<std::mutex> lock(g_mutex);
@@ -868,12 +652,12 @@ int encode_codes(CUtensorMap *m, const QmkKvCache *c, void *codes) {
       enc = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
     }
   }
-  // rows of 32, 64 or 128 bytes as lines of 128, boxes of one tile (Shape::kTile)
+  // rows of 32, 64 or 128 bytes as lines of 128, boxes of `tile` positions
   const cuuint64_t row = (cuuint64_t)c->head_dim * c->bits / 8, head = row * c->capacity;
   const cuuint64_t seq = c->num_seqs > 1 ? (cuuint64_t)c->code_seq_stride : head * c->num_kv_heads;
   const cuuint64_t dims[4] = {128, head / 128, (cuuint64_t)c->num_kv_heads, (cuuint64_t)c->num_seqs};
   const cuuint64_t strides[3] = {128, head, seq};
-  const cuuint32_t box[4] = {128, (cuuint32_t)(row == 128 ? 32 : row / 2), 1, 1}, one[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {128, (cuuint32_t)(tile * row / 128), 1, 1}, one[4] = {1, 1, 1, 1};
   const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, codes, dims, strides, box, one,
                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -882,10 +666,10 @@ int encode_codes(CUtensorMap *m, const QmkKvCache *c, void *codes) {
 }
 
 template <typename... KArgs, typename... Args>
-cudaError_t launch_pdl(void (*kernel)(KArgs...), int grid, int block, size_t smem, cudaStream_t stream,
+cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, int block, size_t smem, cudaStream_t stream,
                        const Args &...args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(block);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
@@ -904,6 +688,10 @@ int tiles_n(int dtype, int max_rows, int ratio) {
 }
 int slots_of(int dtype, int nt) { return nt * (dtype == QMK_FP32 ? 4 : 8); }
 
+// Where the tcgen05 kernel takes over: its 128 query lines cost the same
+// however few are used.
+bool use_tc(int dtype, int max_rows, int ratio) { return dtype != QMK_FP32 && (long long)max_rows * ratio >= 64; }
+
 int check_attend(const char *who, const QmkKvCache *c, const QmkKvRows *r, int num_q_heads, int dtype) {
   int rc = check_cache(who, c);
   if (rc == QMK_OK) rc = check_rows(who, c, r);
@@ -917,9 +705,19 @@ int check_attend(const char *who, const QmkKvCache *c, const QmkKvRows *r, int n
 }
 
 size_t workspace_need(const QmkKvCache *c, const QmkKvRows *r, int num_q_heads, int dtype) {
-  const int slots = slots_of(dtype, tiles_n(dtype, r->max_rows, num_q_heads / c->num_kv_heads));
-  const size_t parts = (size_t)kMaxWorkers * 2 * slots * (c->head_dim + 4) * 4;
+  const int ratio = num_q_heads / c->num_kv_heads;
+  const bool tc = use_tc(dtype, r->max_rows, ratio);
+  const int slots = tc ? 128 : slots_of(dtype, tiles_n(dtype, r->max_rows, ratio));
+  const size_t parts = (size_t)(tc ? kMaxSms : kMaxWorkers) * 2 * slots * (c->head_dim + 4) * 4;
   return kDescBytes + (parts + 255) / 256 * 256;
+}
+
+template <typename T, int D>
+cudaError_t launch_merge(const AttendArgs &a, int workers, int slots, int sms, cudaStream_t stream) {
+  int rb, hb, head_blocks;
+  block_shape(slots, a.ratio, rb, hb, head_blocks);
+  return launch_pdl(merge_kernel<T, D>, dim3(std::min(workers, 4 * sms), (slots + 15) / 16), 32 * kMergeWarps, 0,
+                    stream, (const int *)a.desc, (const float *)a.parts, workers, slots, hb, a.out, a.o_row, a.o_head);
 }
 
 template <typename T, int BITS, int D, int NT>
@@ -935,14 +733,17 @@ int launch_attend(AttendArgs &a, int sms, int dev, cudaStream_t stream) {
       ready[dev] = true;
     }
   }
-  const int grid = std::min(sms, kMaxSms);
-  int rb, hb, head_blocks;
-  block_shape(S::kSlots, a.ratio, rb, hb, head_blocks);
-  cudaError_t e = launch_pdl(attend_kernel<T, BITS, D, NT>, grid, 32 * S::kWarps, S::kSmem, stream, a);
+  cudaError_t e = launch_pdl(attend_kernel<T, BITS, D, NT>, dim3(sms), 32 * S::kWarps, S::kSmem, stream, a);
+  if (e == cudaSuccess) e = launch_merge<T, D>(a, sms * S::kWarps, S::kSlots, sms, stream);
+  if (e != cudaSuccess) return fail(QMK_ERR_CUDA, "qmk_kv_attend launch: %s", cudaGetErrorString(e));
+  return QMK_OK;
+}
+
+template <typename T>
+int launch_tc_attend(const QmkKvCache *c, AttendArgs &a, int dtype, int sms, int dev, cudaStream_t stream) {
+  cudaError_t e = attend_tc(a, dtype, c->bits, c->head_dim, sms, dev, stream);
   if (e == cudaSuccess)
-    e = launch_pdl(merge_kernel<T, D>, std::min(grid * S::kWarps, 4 * sms), 32 * kMergeWarps, 0, stream,
-                   (const int *)a.desc, (const float *)a.parts, grid * S::kWarps, (int)S::kSlots, hb, a.out, a.o_row,
-                   a.o_head);
+    e = c->head_dim == 128 ? launch_merge<T, 128>(a, sms, 128, sms, stream) : launch_merge<T, 64>(a, sms, 128, sms, stream);
   if (e != cudaSuccess) return fail(QMK_ERR_CUDA, "qmk_kv_attend launch: %s", cudaGetErrorString(e));
   return QMK_OK;
 }
@@ -989,9 +790,12 @@ extern "C" int qmk_kv_attend(const QmkKvCache *cache, const QmkKvRows *rows, con
   if (e == cudaSuccess && (dev < 0 || dev >= kMaxDevices)) e = cudaErrorInvalidDevice;
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return fail(QMK_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
+  sms = std::min(sms, kMaxSms);
   AttendArgs a;
-  rc = encode_codes(&a.k_map, cache, cache->k_codes);
-  if (rc == QMK_OK) rc = encode_codes(&a.v_map, cache, cache->v_codes);
+  const bool tc = use_tc(q->dtype, rows->max_rows, num_q_heads / cache->num_kv_heads);
+  const int tile = tc ? 128 : cache->head_dim * cache->bits == 1024 ? 32 : 64;  // Shape::kTile
+  rc = encode_codes(&a.k_map, cache, cache->k_codes, tile);
+  if (rc == QMK_OK) rc = encode_codes(&a.v_map, cache, cache->v_codes, tile);
   if (rc != QMK_OK) return rc;
   a.k_scales = static_cast<const __nv_bfloat16 *>(cache->k_scales);
   a.v_scales = static_cast<const __nv_bfloat16 *>(cache->v_scales);
@@ -1007,10 +811,14 @@ extern "C" int qmk_kv_attend(const QmkKvCache *cache, const QmkKvRows *rows, con
   a.o_row = out->row_stride;
   a.o_head = out->head_stride;
   a.q_aligned = vector_aligned(q);
+  a.o_aligned = vector_aligned(out);
   a.scale_log2 = scale * kLog2e;
   a.desc = static_cast<int *>(workspace);
   a.parts = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + kDescBytes);
   a.status = status;
+  if (tc)
+    return q->dtype == QMK_BF16 ? launch_tc_attend<__nv_bfloat16>(cache, a, QMK_BF16, sms, dev, stream)
+                                : launch_tc_attend<__half>(cache, a, QMK_FP16, sms, dev, stream);
   const int nt = tiles_n(q->dtype, rows->max_rows, a.ratio);
   if (q->dtype == QMK_BF16) return pick_format<__nv_bfloat16>(cache, a, nt, sms, dev, stream);
   if (q->dtype == QMK_FP16) return pick_format<__half>(cache, a, nt, sms, dev, stream);
