@@ -573,12 +573,13 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const int *__re
         float x[8][kPer];
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
-          const int k = min(k0 + q * share, np - 1);
+          const int k = k0 + q * share;
+          ml[q] = make_float2(-INFINITY, 0.f);
+          if (k >= np) continue;
           const float *p = p0 + k * step + (k == 0 ? 0 : tail);
           ml[q] = __ldcg(reinterpret_cast<const float2 *>(p - kPer * lane + D));
           if constexpr (kPer == 4) *reinterpret_cast<float4 *>(x[q]) = __ldcg(reinterpret_cast<const float4 *>(p));
           else *reinterpret_cast<float2 *>(x[q]) = __ldcg(reinterpret_cast<const float2 *>(p));
-          if (k0 + q * share >= np) ml[q] = make_float2(-INFINITY, 0.f);
         }
         float mn = M;
 #pragma unroll
@@ -707,7 +708,7 @@ int check_attend(const char *who, const QmkKvCache *c, const QmkKvRows *r, int n
 size_t workspace_need(const QmkKvCache *c, const QmkKvRows *r, int num_q_heads, int dtype) {
   const int ratio = num_q_heads / c->num_kv_heads;
   const bool tc = use_tc(dtype, r->max_rows, ratio);
-  const int slots = tc ? 128 : slots_of(dtype, tiles_n(dtype, r->max_rows, ratio));
+  const int slots = tc ? kTcLines : slots_of(dtype, tiles_n(dtype, r->max_rows, ratio));
   const size_t parts = (size_t)(tc ? kMaxSms : kMaxWorkers) * 2 * slots * (c->head_dim + 4) * 4;
   return kDescBytes + (parts + 255) / 256 * 256;
 }
@@ -743,7 +744,8 @@ template <typename T>
 int launch_tc_attend(const QmkKvCache *c, AttendArgs &a, int dtype, int sms, int dev, cudaStream_t stream) {
   cudaError_t e = attend_tc(a, dtype, c->bits, c->head_dim, sms, dev, stream);
   if (e == cudaSuccess)
-    e = c->head_dim == 128 ? launch_merge<T, 128>(a, sms, 128, sms, stream) : launch_merge<T, 64>(a, sms, 128, sms, stream);
+    e = c->head_dim == 128 ? launch_merge<T, 128>(a, sms, kTcLines, sms, stream)
+                           : launch_merge<T, 64>(a, sms, kTcLines, sms, stream);
   if (e != cudaSuccess) return fail(QMK_ERR_CUDA, "qmk_kv_attend launch: %s", cudaGetErrorString(e));
   return QMK_OK;
 }

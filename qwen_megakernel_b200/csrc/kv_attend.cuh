@@ -11,6 +11,7 @@ namespace qkv {
 
 using namespace qmk;
 
+constexpr int kTcLines = 256;  // query lines of an item of kv_attend_tc.cu
 constexpr unsigned long long kWaitNs = 1000000000ull;  // bound on one wait
 
 struct AttendArgs {
@@ -46,27 +47,32 @@ struct Segment {
   long long units;       // tiles of one (K/V head, head block)
 };
 
-// sum of floor((a i + b) / m) over i < n, by the Euclidean exchange of a and m
-__device__ inline long long floor_sum(long long n, unsigned m, unsigned a, unsigned b) {
-  long long sum = 0;
-  unsigned k = (unsigned)n;
-  while (k > 0) {
-    if (a >= m) {
-      sum += (long long)(k - 1) * k / 2 * (a / m);
-      a %= m;
-    }
-    if (b >= m) {
-      sum += (long long)k * (b / m);
-      b %= m;
-    }
-    const unsigned long long y = (unsigned long long)a * k + b;
+// a / b of values that are rarely past 32 bits (a 64-bit division is ten times a 32-bit one)
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return (unsigned)a / (unsigned)b;
+  return a / b;
+}
+
+// sum of floor((a i + b) / m) over i < k, by the Euclidean exchange of a and
+// m; the first step by itself, for M is a power of two.  a < 2^9, b < 2^31, k
+// a k + b below 2^31 + 2^25.
+template <unsigned M>
+__device__ inline long long floor_sum(unsigned k, unsigned a, unsigned b) {
+  if (k == 0) return 0;
+  long long sum = (long long)(k - 1) * k / 2 * (a / M) + (long long)k * (b / M);
+  unsigned m = M;
+  a %= M;
+  b %= M;
+  while (a > 0) {
+    const unsigned y = a * k + b;  // (a, b < m <= 2^9, k < 2^17)
     if (y < m) break;
-    const unsigned nk = (unsigned)(y / m);
-    b = (unsigned)(y % m);
-    k = nk;
+    k = y / m;
+    b = y % m;
     const unsigned t = m;
     m = a;
-    a = t;
+    a = t % m;
+    sum += (long long)(k - 1) * k / 2 * (t / m) + (long long)k * (b / m);
+    b %= m;
   }
   return sum;
 }
@@ -76,7 +82,7 @@ template <int TILE>
 __device__ inline long long block_prefix(const Segment &s, int rb, int cb) {
   long long u = 0;
   const int whole = min(cb, s.ok_blocks - 1);  // the last block in range may be cut
-  if (whole > 0) u = floor_sum(whole, TILE, rb, s.start + rb + TILE - 1);
+  if (whole > 0) u = floor_sum<TILE>(whole, rb, s.start + rb + TILE - 1);
   if (cb >= s.ok_blocks && s.ok_blocks > 0) u += (s.start + s.ok_rows + TILE - 1) / TILE;
   return u + max(0, cb - s.ok_blocks);  // a block out of range: one empty tile
 }
@@ -143,8 +149,8 @@ __device__ inline Range find_range(const Rows &R, int rb, int per_seg, long long
   s_before[tid] += base;
   __syncthreads();
   r.workers = max(1ll, min(most, r.total));
-  r.u0 = me < r.workers ? me * r.total / r.workers : 0;
-  r.u1 = me < r.workers ? (me + 1) * r.total / r.workers : 0;
+  r.u0 = me < r.workers ? quotient(me * r.total, r.workers) : 0;
+  r.u1 = me < r.workers ? quotient((me + 1) * r.total, r.workers) : 0;
   // the last thread whose count starts at or before u0 (equal starts are
   // segments without rows; threads past the last segment start at `total`)
   int at = 0;
@@ -179,7 +185,7 @@ __device__ inline Item next_item(const Rows &R, Range &r, Segment &s, int rb, in
   }
   Item it;
   const long long in_seg = r.u0 - r.seg_at;
-  const int hh = (int)(in_seg / s.units);
+  const int hh = (int)quotient(in_seg, s.units);
   it.h = hh / head_blocks;
   it.head0 = (hh - it.h * head_blocks) * hb;
   const long long in_head = in_seg - (long long)hh * s.units;
@@ -209,7 +215,7 @@ __device__ __forceinline__ void describe_cut(int *desc, const Item &it, const Se
   desc[3] = it.h * ratio + it.head0;
   desc[4] = min(hb, ratio - it.head0);
   // parts: this worker's and those up to the worker with the item's last tile
-  desc[0] = (int)(((it.u0 + it.tiles) * r.workers - 1) / r.total - me) + 1;
+  desc[0] = (int)(quotient((it.u0 + it.tiles) * r.workers - 1, r.total) - me) + 1;
 }
 
 // ------------------------------------------------------------- instructions
@@ -278,7 +284,7 @@ __device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, i
 
 // Host: kv_attend.cu.
 int check_attend(const char *who, const QmkKvCache *c, const QmkKvRows *r, int num_q_heads, int dtype);
-// kv_attend_tc.cu: dtype QMK_BF16 or QMK_FP16; parts of 128 slots a worker (CTA).
+// kv_attend_tc.cu: dtype QMK_BF16 or QMK_FP16; parts of kTcLines slots a worker (CTA).
 cudaError_t attend_tc(const AttendArgs &a, int dtype, int bits, int head_dim, int grid, int dev, cudaStream_t stream);
 
 }  // namespace qkv
