@@ -503,6 +503,25 @@ int qmk_kv_attend(const QmkKvCache *cache, const QmkKvRows *rows, const QmkKvTen
                   const QmkKvTensor *out, float scale, void *workspace, size_t workspace_bytes,
                   unsigned int *status, cudaStream_t stream);
 
+/* ---- the token-parallel forward pass over a quantized cache --------------
+ * qmk_batch_forward with the K/V rows held by a quantized cache: each layer's
+ * K (after norm and RoPE) and V are quantized as they are written, and the
+ * attention is qmk_kv_attend.  args->k_cache, v_cache, kv_seq_stride and
+ * causal_run are not used; kvq->cache describes layer 0 (8 K/V heads,
+ * head_dim 128) of num_layers, kvq->rows the args' rows in segments
+ * (rows.rows == num_rows; row_seq and row_pos must say the same). */
+typedef struct QmkBatchKvq {
+  QmkKvCache cache;
+  long long code_layer_stride;   /* bytes, a multiple of 16                   */
+  long long scale_layer_stride;  /* bf16 elements, a multiple of 8            */
+  QmkKvRows rows;
+  void *workspace;               /* qmk_kv_attend_workspace_bytes(&cache,     */
+  size_t workspace_bytes;        /*   &rows, 16, QMK_FP16)                    */
+  unsigned int *status;          /* device uint32 [1] or NULL: QMK_KV_*       */
+} QmkBatchKvq;
+
+int qmk_batch_forward_kvq(const QmkBatchArgs *args, const QmkBatchKvq *kvq, cudaStream_t stream);
+
 /* Library version string. */
 const char *qmk_version(void);
 

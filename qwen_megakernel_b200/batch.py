@@ -25,6 +25,7 @@ import math
 import torch
 
 from . import _native
+from .kv_cache import KVRows, QuantKVCache
 from .weights import HEAD_DIM, NUM_KV_HEADS, TENSORS_PER_LAYER, VOCAB_SIZE
 
 MAX_ROWS = 4096  # QMK_BATCH_MAX_ROWS
@@ -97,6 +98,27 @@ class BatchForward:
             stride, int(num_seqs), self.num_layers, self.max_seq_len, self.attn_scale, tokens, row_seq, row_pos,
             out_rows, out_tokens, logits, self.status, 1 if causal_run else 0)
 
+    def forward_quantized(self, cache, rows, tokens, row_seq, row_pos, out_rows=None, out_tokens=None, logits=None,
+                          workspace=None) -> None:
+        """``forward`` with the K/V rows in ``cache`` (a ``QuantKVCache`` of this
+        model's layers): ``rows`` (a ``KVRows``) holds the same rows as
+        ``row_seq`` and ``row_pos``, in segments."""
+        if (cache.num_layers, cache.num_kv_heads, cache.head_dim) != (self.num_layers, NUM_KV_HEADS, HEAD_DIM):
+            raise ValueError(f"the cache must hold {self.num_layers} layers of {NUM_KV_HEADS} x {HEAD_DIM}")
+        if cache.max_seq_len > self.max_seq_len:
+            raise ValueError(f"the cache's max_seq_len {cache.max_seq_len} exceeds the tables' {self.max_seq_len}")
+        n = int(tokens.numel())
+        cache.check_rows(rows)
+        if rows.rows != n:
+            raise ValueError(f"rows hold {rows.rows} rows for {n} tokens")
+        out = 0 if out_rows is None else int(out_rows.numel())
+        ws = self.workspace(n, out) if workspace is None else workspace
+        self._ops.batch_forward_kvq(
+            ws, self.embed, self.layer_ptrs, self.fused_ptrs, self.final_norm, self.lm_head, self.cos, self.sin,
+            cache.k_codes, cache.v_codes, cache.k_scales, cache.v_scales, cache.bits, cache.max_seq_len,
+            self.attn_scale, tokens, row_seq, row_pos, rows.start, rows.row_offsets, rows.seq, rows.max_rows, out_rows,
+            out_tokens, logits, self.status, cache.status)
+
     def check_status(self) -> None:
         """Raise BatchError if a device-side check fired (after a sync)."""
         code = int(self.status.item())
@@ -127,24 +149,36 @@ class BatchDecoder:
     row per sequence."""
 
     def __init__(self, weights, batch_size: int, max_seq_len: int | None = None, use_graphs: bool = True,
-                 decode: str = "auto"):
+                 decode: str = "auto", kv_bits: int | None = None):
         """decode: "token_parallel" (one row per sequence through the
         token-parallel kernels), "megakernel" (the persistent decode kernel's
         batched instance, B == MEGAKERNEL_SEQS only) or "auto" (the persistent
-        kernel when B == MEGAKERNEL_SEQS)."""
+        kernel when B == MEGAKERNEL_SEQS).
+
+        kv_bits: 4 or 8 holds the K/V rows in a ``QuantKVCache`` (``kv``;
+        ``k_cache`` and ``v_cache`` are None) of 0.28 or 0.53 of the bf16
+        cache's bytes, through the token-parallel kernels at every B."""
         if batch_size < 1 or batch_size > MAX_ROWS:
             raise ValueError(f"batch_size must be in [1, {MAX_ROWS}]")
         if decode not in ("auto", "token_parallel", "megakernel"):
             raise ValueError("decode must be 'auto', 'token_parallel' or 'megakernel'")
         if decode == "megakernel" and batch_size != MEGAKERNEL_SEQS:
             raise ValueError(f"the persistent kernel decodes exactly {MEGAKERNEL_SEQS} sequences")
+        if kv_bits is not None and decode == "megakernel":
+            raise ValueError("the persistent kernel decodes from the bf16 cache: kv_bits needs decode='token_parallel'")
+        if kv_bits not in (None, 4, 8):
+            raise ValueError("kv_bits must be None, 4 or 8")
         self.B = int(batch_size)
         self.fw = BatchForward(weights, int(max_seq_len or weights["cos_table"].shape[0]))
         self.device = self.fw.device
         self.max_seq_len = self.fw.max_seq_len
         shape = (self.B,) + self.fw.cache_shape()
-        self.k_cache = torch.zeros(shape, dtype=torch.bfloat16, device=self.device)
-        self.v_cache = torch.zeros_like(self.k_cache)
+        self.kv = self.k_cache = self.v_cache = None
+        if kv_bits is None:
+            self.k_cache = torch.zeros(shape, dtype=torch.bfloat16, device=self.device)
+            self.v_cache = torch.zeros_like(self.k_cache)
+        else:
+            self.kv = QuantKVCache(self.B, self.max_seq_len, self.fw.num_layers, bits=kv_bits, device=self.device)
         self.positions = [0] * self.B
         self.use_graphs = bool(use_graphs)
         # Static step inputs/outputs (graph-captured addresses).
@@ -155,8 +189,9 @@ class BatchDecoder:
         self._ws_step = torch.empty(int(self.fw._ops.batch_workspace_bytes(self.B, self.B)), dtype=torch.uint8,
                                     device=self.device)
         self._graph = None
-        self.decode_mode = "megakernel" if (decode == "megakernel" or (decode == "auto" and self.B == MEGAKERNEL_SEQS)) \
-            else "token_parallel"
+        self._step_rows = KVRows.from_tensors(self._pos, seq=self._seq)
+        self.decode_mode = "megakernel" if (decode == "megakernel" or (
+            decode == "auto" and self.B == MEGAKERNEL_SEQS and kv_bits is None)) else "token_parallel"
         if self.decode_mode == "megakernel":
             from .model import _pack_layer_weights
 
@@ -170,6 +205,8 @@ class BatchDecoder:
         (persistent kernel) reported a device error; call after a stream
         synchronize."""
         self.fw.check_status()
+        if self.kv is not None:
+            self.kv.check_status()
         if self.decode_mode == "megakernel":
             from .model import _ERROR_NAMES, DecodeError
 
@@ -180,8 +217,11 @@ class BatchDecoder:
                                   f"cta {info >> 16}, site {(info >> 8) & 0xFF}, layer {info & 0xFF}")
 
     def reset(self) -> None:
-        self.k_cache.zero_()
-        self.v_cache.zero_()
+        if self.kv is not None:
+            self.kv.reset()
+        else:
+            self.k_cache.zero_()
+            self.v_cache.zero_()
         self.positions = [0] * self.B
 
     def prefill(self, prompts: list[list[int]], logits: torch.Tensor | None = None) -> list[int]:
@@ -211,7 +251,15 @@ class BatchDecoder:
             lg = None
             if logits is not None and outs:
                 lg = torch.empty(len(outs), VOCAB_SIZE, dtype=torch.float32, device=self.device)
-            self.fw.forward(self.k_cache, self.v_cache, self.B, tokens, row_seq, row_pos, out_rows, out_tok, lg)
+            if self.kv is not None:
+                first = {}  # sequence -> its first position in the chunk (rows run sequence by sequence)
+                for s, p, _ in chunk:
+                    first.setdefault(s, p)
+                counts = [sum(1 for r in chunk if r[0] == s) for s in first]
+                self.fw.forward_quantized(self.kv, KVRows(list(first.values()), counts, list(first), self.device),
+                                          tokens, row_seq, row_pos, out_rows, out_tok, lg)
+            else:
+                self.fw.forward(self.k_cache, self.v_cache, self.B, tokens, row_seq, row_pos, out_rows, out_tok, lg)
             if outs:
                 got = out_tok.cpu().tolist()
                 for (_, s), t in zip(outs, got):
@@ -221,11 +269,17 @@ class BatchDecoder:
                         logits[s].copy_(lg[k])
         torch.cuda.current_stream(self.device).synchronize()
         self.fw.check_status()
+        if self.kv is not None:
+            self.kv.check_status()
         for s, p in enumerate(prompts):
             self.positions[s] += len(p)
         return next_tok
 
     def _launch_step(self, logits=None) -> None:
+        if self.kv is not None:
+            self.fw.forward_quantized(self.kv, self._step_rows, self._tok, self._seq, self._pos, self._seq, self._out,
+                                      logits, workspace=self._ws_step)
+            return
         self.fw.forward(self.k_cache, self.v_cache, self.B, self._tok, self._seq, self._pos, self._seq, self._out,
                         logits, workspace=self._ws_step)
 

@@ -30,6 +30,7 @@
 #include <cstdio>
 #include <mutex>
 
+#include "kv_cache.cuh"
 #include "qmk_device.cuh"
 #include "qwen_megakernel.h"
 
@@ -240,6 +241,107 @@ __global__ void __launch_bounds__(256) qk_rope_kv_kernel(
       make_uint2(*reinterpret_cast<const unsigned *>(&k01), *reinterpret_cast<const unsigned *>(&k23));
   *reinterpret_cast<uint2 *>(v_cache + off) =
       make_uint2(*reinterpret_cast<const unsigned *>(&v01), *reinterpret_cast<const unsigned *>(&v23));
+}
+
+// The same norms and rotation with a quantized cache: K and V are quantized
+// from the fp32 values (a lane's 4 dimensions, 8 lanes a group), the queries
+// leave as fp16 [rows, 16, 128] for qmk_kv_attend (11 bits against the 4 or 8
+// of the keys; unscaled, so that they are of order 1).
+template <int BITS>
+__global__ void __launch_bounds__(256) qk_rope_kvq_kernel(
+    const float *__restrict__ qkv, const __nv_bfloat16 *__restrict__ q_norm, const __nv_bfloat16 *__restrict__ k_norm,
+    const __nv_bfloat16 *__restrict__ cos_t, const __nv_bfloat16 *__restrict__ sin_t, const int *__restrict__ row_seq,
+    const int *__restrict__ row_pos, QmkKvCache cache, __half *__restrict__ q_out, unsigned *status,
+    unsigned *kv_status, int nsplit, long long split_stride) {
+  pdl_wait();  // inputs are written by the previous kernel
+  pdl_trigger();
+  const int r = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int seq = row_seq[r], pos = row_pos[r];
+  if (seq < 0 || seq >= cache.num_seqs || pos < 0 || pos >= cache.max_seq_len) {
+    if (threadIdx.x == 0 && status) atomicOr(status, QMK_BATCH_BAD_ROW);
+    // (the attention gives such a row zeros, whatever its query)
+    reinterpret_cast<uint4 *>(q_out + (size_t)r * kQSize)[threadIdx.x] = make_uint4(0u, 0u, 0u, 0u);
+    return;
+  }
+  const int d0 = 4 * lane;
+  const uint2 cv = __ldg(reinterpret_cast<const uint2 *>(cos_t + (size_t)pos * kHeadDim + d0));
+  const uint2 sv = __ldg(reinterpret_cast<const uint2 *>(sin_t + (size_t)pos * kHeadDim + d0));
+  const float cf[4] = {bf_lo(cv.x), bf_hi(cv.x), bf_lo(cv.y), bf_hi(cv.y)};
+  const float sf[4] = {bf_lo(sv.x), bf_hi(sv.x), bf_lo(sv.y), bf_hi(sv.y)};
+  auto load4 = [&](int col, float (&x)[4]) {  // hi + lo rows of every K-split partial, in split order
+    x[0] = x[1] = x[2] = x[3] = 0.f;
+    for (int sp = 0; sp < nsplit; ++sp) {
+      const float *p = qkv + (size_t)sp * (size_t)split_stride + (size_t)r * kQKV + col;
+      const float4 h = *reinterpret_cast<const float4 *>(p);
+      const float4 l = *reinterpret_cast<const float4 *>(p + (size_t)gridDim.x * kQKV);
+      x[0] += h.x + l.x;
+      x[1] += h.y + l.y;
+      x[2] += h.z + l.z;
+      x[3] += h.w + l.w;
+    }
+  };
+  auto norm_rope = [&](int col, const __nv_bfloat16 *nw, float (&y)[4]) {
+    float x[4];
+    load4(col + d0, x);
+    const float rr =
+        rsqrtf(warp_sum(x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3]) / (float)kHeadDim + kRmsEps);
+    const uint2 wv = __ldg(reinterpret_cast<const uint2 *>(nw + d0));
+    const float wf[4] = {bf_lo(wv.x), bf_hi(wv.x), bf_lo(wv.y), bf_hi(wv.y)};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = (x[e] * rr) * wf[e];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float partner = __shfl_xor_sync(0xffffffffu, x[e], 16);
+      y[e] = (lane < 16) ? (x[e] * cf[e] - partner * sf[e]) : (x[e] * cf[e] + partner * sf[e]);
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int h = warp + 8 * k;
+    float y[4];
+    norm_rope(h * kHeadDim, q_norm, y);
+    const __half2 a = __floats2half2_rn(y[0], y[1]), b = __floats2half2_rn(y[2], y[3]);
+    *reinterpret_cast<uint2 *>(q_out + (size_t)r * kQSize + h * kHeadDim + d0) =
+        make_uint2(*reinterpret_cast<const unsigned *>(&a), *reinterpret_cast<const unsigned *>(&b));
+  }
+  const size_t at = (size_t)warp * (size_t)cache.capacity + (size_t)pos;
+  auto store = [&](const float (&x)[4], void *codes, void *scales) {
+    unsigned word[1];
+    const __nv_bfloat16 s = qkv::quantize<BITS, 4>(x, word, kv_status);
+    uint8_t *c = static_cast<uint8_t *>(codes) + (size_t)seq * (size_t)cache.code_seq_stride +
+                 at * (kHeadDim * BITS / 8) + lane * BITS / 2;
+    if constexpr (BITS == 4) *reinterpret_cast<unsigned short *>(c) = (unsigned short)word[0];
+    else *reinterpret_cast<unsigned *>(c) = word[0];
+    if ((lane & 7) == 0)
+      static_cast<__nv_bfloat16 *>(scales)[(size_t)seq * (size_t)cache.scale_seq_stride + at * (kHeadDim / 32) +
+                                           (lane >> 3)] = s;
+  };
+  float y[4];
+  norm_rope(kQSize + warp * kHeadDim, k_norm, y);
+  store(y, cache.k_codes, cache.k_scales);
+  load4(kQSize + kKVSize + warp * kHeadDim + d0, y);
+  store(y, cache.v_codes, cache.v_scales);
+}
+
+// The fp16 attention output [R, 2048] as the stacked O-projection input (a bf16
+// pair holds an fp16 value exactly).  Grid: rows, 256 threads, 8 values each.
+__global__ void __launch_bounds__(256) att_split_kernel(const __half *__restrict__ att,
+                                                        __nv_bfloat16 *__restrict__ a2) {
+  pdl_wait();  // inputs are written by the previous kernel
+  pdl_trigger();
+  const int r = blockIdx.x, R = gridDim.x, c = 8 * threadIdx.x;
+  const uint4 w = *reinterpret_cast<const uint4 *>(att + (size_t)r * kQSize + c);
+  const __half *e = reinterpret_cast<const __half *>(&w);
+  uint2 hi[2], lo[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const float y[4] = {__half2float(e[4 * k]), __half2float(e[4 * k + 1]), __half2float(e[4 * k + 2]),
+                        __half2float(e[4 * k + 3])};
+    split4(y, hi[k], lo[k]);
+  }
+  *reinterpret_cast<uint4 *>(a2 + (size_t)r * kQSize + c) = make_uint4(hi[0].x, hi[0].y, hi[1].x, hi[1].y);
+  *reinterpret_cast<uint4 *>(a2 + (size_t)(R + r) * kQSize + c) = make_uint4(lo[0].x, lo[0].y, lo[1].x, lo[1].y);
 }
 
 // GQA attention of row r over positions [0, row_pos[r]] of its sequence's
@@ -894,12 +996,16 @@ extern "C" size_t qmk_batch_workspace_bytes(int num_rows, int num_out) {
   return layout(num_rows, num_out).total;
 }
 
-extern "C" int qmk_batch_forward(const QmkBatchArgs *a, cudaStream_t stream) {
+namespace {
+
+// The forward pass; K/V in the bf16 caches of `a`, or in the quantized cache
+// `kvq` if given.
+int forward(const QmkBatchArgs *a, const QmkBatchKvq *kvq, cudaStream_t stream) {
   using namespace qmb;
   qmk_internal_clear_error();
   if (!a) return fail(QMK_ERR_ARGS, "qmk_batch_forward: null args");
   if (!a->embed_weight || !a->layer_ptrs || !a->final_norm_weight || !a->lm_head_weight || !a->cos_table ||
-      !a->sin_table || !a->k_cache || !a->v_cache || !a->tokens || !a->row_seq || !a->row_pos)
+      !a->sin_table || (!kvq && (!a->k_cache || !a->v_cache)) || !a->tokens || !a->row_seq || !a->row_pos)
     return fail(QMK_ERR_ARGS, "qmk_batch_forward: null weight/table/cache/row pointer");
   if (a->num_rows < 1 || a->num_rows > QMK_BATCH_MAX_ROWS)
     return fail(QMK_ERR_ARGS, "qmk_batch_forward: num_rows=%d outside [1, %d]", a->num_rows, QMK_BATCH_MAX_ROWS);
@@ -911,16 +1017,39 @@ extern "C" int qmk_batch_forward(const QmkBatchArgs *a, cudaStream_t stream) {
   if (a->max_seq_len < 1 || a->num_seqs < 1)
     return fail(QMK_ERR_ARGS, "qmk_batch_forward: max_seq_len=%d num_seqs=%d", a->max_seq_len, a->num_seqs);
   const long long per_seq = (long long)a->num_layers * kNumKVHeads * a->max_seq_len * kHeadDim;
-  if (a->num_seqs > 1 && a->kv_seq_stride < per_seq)
+  if (!kvq && a->num_seqs > 1 && a->kv_seq_stride < per_seq)
     return fail(QMK_ERR_ARGS, "qmk_batch_forward: kv_seq_stride=%lld < one cache (%lld elements)", a->kv_seq_stride,
                 per_seq);
   // The attention copies cache rows with 1-D bulk copies: 16-byte aligned
   // sources (cache bases and the per-sequence stride).
-  if ((reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->v_cache)) % 16)
+  if (!kvq && (reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->v_cache)) % 16)
     return fail(QMK_ERR_ARGS, "qmk_batch_forward: k_cache / v_cache not 16-byte aligned");
-  if (a->num_seqs > 1 && a->kv_seq_stride % 8)
+  if (!kvq && a->num_seqs > 1 && a->kv_seq_stride % 8)
     return fail(QMK_ERR_ARGS, "qmk_batch_forward: kv_seq_stride=%lld not a multiple of 8 elements (16 bytes)",
                 a->kv_seq_stride);
+  if (kvq) {
+    const char *who = "qmk_batch_forward_kvq";
+    const QmkKvCache &c = kvq->cache;
+    int rc = qkv::check_cache(who, &c);
+    if (rc == QMK_OK) rc = qkv::check_rows(who, &c, &kvq->rows);
+    if (rc != QMK_OK) return rc;
+    if (c.num_kv_heads != kNumKVHeads || c.head_dim != kHeadDim || c.num_seqs != a->num_seqs ||
+        c.max_seq_len != a->max_seq_len)
+      return fail(QMK_ERR_ARGS, "%s: the cache is not one of num_seqs=%d, %d heads, max_seq_len=%d, head_dim %d", who,
+                  a->num_seqs, kNumKVHeads, a->max_seq_len, kHeadDim);
+    if (kvq->rows.rows != a->num_rows || kvq->rows.segments < 1 || kvq->rows.max_rows < 1)
+      return fail(QMK_ERR_ARGS, "%s: %d rows in %d segments of up to %d for num_rows=%d", who, kvq->rows.rows,
+                  kvq->rows.segments, kvq->rows.max_rows, a->num_rows);
+    const long long rows = (long long)c.num_kv_heads * c.capacity;
+    if (a->num_layers > 1 &&
+        (kvq->code_layer_stride < rows * (c.head_dim * c.bits / 8) || kvq->code_layer_stride % 16 ||
+         kvq->scale_layer_stride < rows * (c.head_dim / 32) || kvq->scale_layer_stride % 8))
+      return fail(QMK_ERR_ARGS, "%s: layer strides smaller than a layer or not multiples of 16 bytes", who);
+    const size_t need = qmk_kv_attend_workspace_bytes(&c, &kvq->rows, kNumQHeads, QMK_FP16);
+    if (need == 0) return QMK_ERR_ARGS;  // (recorded)
+    if (!kvq->workspace || kvq->workspace_bytes < need || reinterpret_cast<uintptr_t>(kvq->workspace) % kAlign)
+      return fail(QMK_ERR_WORKSPACE, "%s: kvq workspace needs %zu bytes, 256-byte aligned", who, need);
+  }
   for (int i = 0; i < a->num_layers * 11; ++i)
     if (!a->layer_ptrs[i]) return fail(QMK_ERR_ARGS, "qmk_batch_forward: layer pointer %d is null", i);
   const Layout Lw = layout(a->num_rows, a->num_out);
@@ -995,6 +1124,23 @@ extern "C" int qmk_batch_forward(const QmkBatchArgs *a, cudaStream_t stream) {
       if (rc == QMK_OK) rc = gemm(R2, kKVSize, kHidden, P[3], a2, qkv2 + kQSize + kKVSize, kQKV, s_qkv, qkv_stride);
     }
     if (rc != QMK_OK) break;
+    if (kvq) {
+      // q and the attention's output, fp16, share the place of the fp32 q
+      QmkKvCache c = kvq->cache;
+      c.k_codes = static_cast<uint8_t *>(c.k_codes) + l * kvq->code_layer_stride;
+      c.v_codes = static_cast<uint8_t *>(c.v_codes) + l * kvq->code_layer_stride;
+      c.k_scales = static_cast<__nv_bfloat16 *>(c.k_scales) + l * kvq->scale_layer_stride;
+      c.v_scales = static_cast<__nv_bfloat16 *>(c.v_scales) + l * kvq->scale_layer_stride;
+      __half *q16 = reinterpret_cast<__half *>(q), *att16 = q16 + (size_t)R * kQSize;
+      launch_pdl(c.bits == 4 ? qk_rope_kvq_kernel<4> : qk_rope_kvq_kernel<8>, dim3(R), dim3(256), 0, stream, qkv2,
+                 bf(P[4]), bf(P[5]), cos_t, sin_t, a->row_seq, a->row_pos, c, q16, a->status, kvq->status, s_qkv,
+                 qkv_stride);
+      const QmkKvTensor qt{q16, QMK_FP16, kQSize, kHeadDim}, ot{att16, QMK_FP16, kQSize, kHeadDim};
+      rc = qmk_kv_attend(&c, &kvq->rows, &qt, kNumQHeads, &ot, a->attn_scale, kvq->workspace, kvq->workspace_bytes,
+                         kvq->status, stream);
+      if (rc != QMK_OK) break;
+      launch_pdl(att_split_kernel, dim3(R), dim3(256), 0, stream, att16, a2);
+    } else {
     launch_pdl(qk_rope_kv_kernel, dim3(R), dim3(256), 0, stream, qkv2, bf(P[4]), bf(P[5]), cos_t, sin_t, a->row_seq, a->row_pos, kc, vc,
                                             a->kv_seq_stride, a->num_seqs, l, a->max_seq_len,
                                             a->attn_scale * kLog2e, q, a->status, s_qkv, qkv_stride);
@@ -1021,6 +1167,7 @@ extern "C" int qmk_batch_forward(const QmkBatchArgs *a, cudaStream_t stream) {
           a->status);
       if (splits > 1) launch_pdl(merge_kernel, dim3(dim3(kNumKVHeads, R)), dim3(64), 0, stream, partial, splits, a2);
     }
+    }
     rc = gemm(R2, kHidden, kQSize, P[6], a2, c2, kHidden, ks, ks_stride);
     if (rc != QMK_OK) break;
     launch_pdl(residual_norm_split_kernel, dim3(R), dim3(256), 0, stream, x, c2, nullptr, R, bf(P[7]), a2, ks, ks_stride);  // x += O-proj
@@ -1046,4 +1193,13 @@ extern "C" int qmk_batch_forward(const QmkBatchArgs *a, cudaStream_t stream) {
   e = cudaGetLastError();
   if (e != cudaSuccess) return fail(QMK_ERR_CUDA, "qmk_batch_forward launch: %s", cudaGetErrorString(e));
   return QMK_OK;
+}
+
+}  // namespace
+
+extern "C" int qmk_batch_forward(const QmkBatchArgs *a, cudaStream_t stream) { return forward(a, nullptr, stream); }
+
+extern "C" int qmk_batch_forward_kvq(const QmkBatchArgs *a, const QmkBatchKvq *kvq, cudaStream_t stream) {
+  if (!kvq) return fail(QMK_ERR_ARGS, "qmk_batch_forward_kvq: null kvq");
+  return forward(a, kvq, stream);
 }

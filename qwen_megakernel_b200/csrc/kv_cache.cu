@@ -126,83 +126,6 @@ __device__ __forceinline__ int fill_rows(RowTable &t, const Args<T> &a, int row0
   return n;
 }
 
-__device__ __forceinline__ float fast_rcp(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// x / s, correctly rounded for what is asked here, from r ~ 1 / s: one Newton
-// step on the quotient with its exact remainder (Markstein's division).  Its
-// error before the last rounding is below 2^-44 of the quotient, so a quotient
-// that fp32 holds (the border of two codes, or of two bf16 scales, among them)
-// comes out exactly, and one that lies off a border is not rounded onto it: x
-// and s have 24 and 8 bits, the nearest such quotient is more than half a step
-// of fp32 away.  Both within 2^-100 .. 2^126.
-__device__ __forceinline__ float divide(float x, float s, float r) {
-  const float q = x * r;
-  return fmaf(fmaf(-q, s, x), r, q);
-}
-
-// 8 values of a group to codes, words packed; any scale, any value.
-template <int BITS>
-__device__ __forceinline__ void codes_any(const float (&x)[8], float s, unsigned (&word)[BITS / 4]) {
-  constexpr float kTop = BITS == 4 ? 7.f : 127.f, kOffset = BITS == 4 ? 8.f : 128.f;
-#pragma unroll
-  for (int i = 0; i < BITS / 4; ++i) word[i] = 0u;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float c = 0.f;
-    if (s != 0.f && x[i] == x[i]) c = fminf(fmaxf(rintf(__fdiv_rn(x[i], s)), -kTop), kTop);
-    word[i * BITS / 32] |= (unsigned)(int)(c + kOffset) << (i * BITS % 32);
-  }
-}
-
-// Codes and scale of a thread's 8 values; the 4 lanes of a group agree.
-template <int BITS>
-__device__ __forceinline__ __nv_bfloat16 quantize8(const float (&x)[8], unsigned (&word)[BITS / 4], unsigned *status) {
-  constexpr float kTop = BITS == 4 ? 7.f : 127.f;
-  unsigned top = 0;  // bits of the largest magnitude, infinities and NaN above all
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-  // largest magnitude within 2^-90 .. 2^126: scale and quotients are ordinary numbers
-  const bool easy = top >= 0x12800000u && top < 0x7e800000u;
-  if (__all_sync(0xffffffffu, easy)) {
-    const __nv_bfloat16 sb = __float2bfloat16_rn(divide(__uint_as_float(top), kTop, 1.f / kTop));
-    const float s = __bfloat162float(sb), r = fast_rcp(s);
-    // x / s + 1.5 2^23 + offset holds the code, rounded to even, in its low
-    // bits; in a word's sum the patterns above the codes add up to a constant
-    constexpr float kMagic = 12582912.f + (BITS == 4 ? 8.f : 128.f);
-    constexpr int kPer = 32 / BITS;
-    unsigned above = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) above += 0x4b400000u << (BITS * i);
-#pragma unroll
-    for (int w = 0; w < BITS / 4; ++w) {
-      unsigned sum = 0u - above;
-#pragma unroll
-      for (int i = 0; i < kPer; ++i)
-        sum += __float_as_uint(divide(x[kPer * w + i], s, r) + kMagic) * (1u << (BITS * i));
-      word[w] = sum;
-    }
-    return sb;
-  }
-  unsigned fin = 0;  // largest finite magnitude
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const unsigned u = __float_as_uint(x[i]) & 0x7fffffffu;
-    fin = max(fin, u < 0x7f800000u ? u : 0u);
-  }
-  fin = max(fin, __shfl_xor_sync(0xffffffffu, fin, 1));
-  fin = max(fin, __shfl_xor_sync(0xffffffffu, fin, 2));
-  if (top >= 0x7f800000u && status) atomicOr(status, QMK_KV_NONFINITE);
-  const __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(__uint_as_float(fin), kTop));
-  codes_any<BITS>(x, __bfloat162float(sb), word);
-  return sb;
-}
-
 // 8 elements as they lie in memory; single loads unless VEC.
 template <typename T, bool VEC>
 struct Raw {
@@ -272,7 +195,7 @@ __global__ void __launch_bounds__(kThreads) write_kernel(const __grid_constant__
           float x[8];
           unsigned word[BITS / 4];
           raw[k][i].get(x);
-          const __nv_bfloat16 sb = quantize8<BITS>(x, word, a.status);
+          const __nv_bfloat16 sb = quantize<BITS, 8>(x, word, a.status);
           if (ok[k]) {
             const int r = r0 + k * lines + line;
             uint8_t *dst = codes[i] + tab.code[r];

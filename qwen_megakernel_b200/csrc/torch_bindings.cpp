@@ -20,6 +20,8 @@
 //   trace_words()        -> qmk_trace_words
 //   kv_write / kv_read / kv_attend -> qmk_kv_write / qmk_kv_read / qmk_kv_attend:
 //                           the quantized K/V cache
+//   batch_forward_kvq    -> qmk_batch_forward_kvq: the token-parallel forward
+//                           pass over a quantized cache
 #include <Python.h>
 
 #include <c10/cuda/CUDAGuard.h>
@@ -635,6 +637,101 @@ void kv_attend(torch::Tensor k_codes, torch::Tensor v_codes, torch::Tensor k_sca
                                c.status, c10::cuda::getCurrentCUDAStream().stream()));
 }
 
+// The token-parallel forward pass over a quantized cache.
+void batch_forward_kvq(torch::Tensor workspace, torch::Tensor embed_weight, std::vector<int64_t> layer_ptrs,
+                       std::vector<int64_t> fused_ptrs, torch::Tensor final_norm_weight, torch::Tensor lm_head_weight,
+                       torch::Tensor cos_table, torch::Tensor sin_table, torch::Tensor k_codes, torch::Tensor v_codes,
+                       torch::Tensor k_scales, torch::Tensor v_scales, int64_t bits, int64_t max_seq_len,
+                       double attn_scale, torch::Tensor tokens, torch::Tensor row_seq, torch::Tensor row_pos,
+                       torch::Tensor start, std::optional<torch::Tensor> row_offsets, std::optional<torch::Tensor> seq,
+                       int64_t max_rows, std::optional<torch::Tensor> out_rows,
+                       std::optional<torch::Tensor> out_tokens, std::optional<torch::Tensor> logits,
+                       std::optional<torch::Tensor> status, std::optional<torch::Tensor> kv_status) {
+  check_dtype(embed_weight, torch::kBFloat16, "embed_weight", "bfloat16");
+  for (const auto *t : {&workspace, &final_norm_weight, &lm_head_weight, &cos_table, &sin_table, &k_codes, &tokens,
+                        &row_seq, &row_pos}) {
+    QMK_CHECK(t->is_cuda() && t->device() == embed_weight.device(), "all tensors must be on the weights' device");
+    QMK_CHECK(t->is_contiguous(), "tensors must be contiguous");
+  }
+  check_dtype(final_norm_weight, torch::kBFloat16, "final_norm_weight", "bfloat16");
+  check_dtype(lm_head_weight, torch::kBFloat16, "lm_head_weight", "bfloat16");
+  check_dtype(cos_table, torch::kBFloat16, "cos_table", "bfloat16");
+  check_dtype(sin_table, torch::kBFloat16, "sin_table", "bfloat16");
+  check_dtype(tokens, torch::kInt32, "tokens", "int32");
+  check_dtype(row_seq, torch::kInt32, "row_seq", "int32");
+  check_dtype(row_pos, torch::kInt32, "row_pos", "int32");
+  const int64_t R = tokens.numel();
+  QMK_CHECK(row_seq.numel() == R && row_pos.numel() == R, "tokens, row_seq and row_pos must have equal length");
+  const KvCall c = kv_call(k_codes, v_codes, k_scales, v_scales, bits, max_seq_len, 0, R, start, row_offsets, seq,
+                           max_rows, kv_status);
+  const int64_t num_layers = k_codes.size(1);
+  QMK_CHECK((int64_t)layer_ptrs.size() == num_layers * 11, "layer_ptrs must hold num_layers * 11 pointers");
+  QMK_CHECK(fused_ptrs.empty() || (int64_t)fused_ptrs.size() == num_layers * 2,
+            "fused_ptrs must be empty or hold num_layers * 2 pointers");
+  QMK_CHECK(cos_table.size(0) >= max_seq_len && sin_table.size(0) >= max_seq_len,
+            "RoPE tables need >= max_seq_len rows");
+  QmkBatchArgs a;
+  memset(&a, 0, sizeof(a));
+  int64_t O = 0;
+  if (out_rows.has_value()) {
+    check_dtype(*out_rows, torch::kInt32, "out_rows", "int32");
+    check_same_device(*out_rows, embed_weight, "out_rows");
+    O = out_rows->numel();
+    a.out_rows = static_cast<const int *>(out_rows->data_ptr());
+  }
+  if (out_tokens.has_value()) {
+    check_dtype(*out_tokens, torch::kInt32, "out_tokens", "int32");
+    check_same_device(*out_tokens, embed_weight, "out_tokens");
+    QMK_CHECK(out_tokens->numel() >= O, "out_tokens must have >= len(out_rows) elements");
+    a.out_tokens = static_cast<int *>(out_tokens->data_ptr());
+  }
+  if (logits.has_value()) {
+    check_dtype(*logits, torch::kFloat32, "logits", "float32");
+    check_same_device(*logits, embed_weight, "logits");
+    QMK_CHECK(logits->numel() >= O * QMK_VOCAB, "logits must hold >= len(out_rows) * %d elements", QMK_VOCAB);
+    a.logits = static_cast<float *>(logits->data_ptr());
+  }
+  if (status.has_value()) {
+    check_dtype(*status, torch::kInt32, "status", "int32");
+    check_same_device(*status, embed_weight, "status");
+    a.status = reinterpret_cast<unsigned *>(status->data_ptr());
+  }
+  std::vector<const void *> ptrs(layer_ptrs.size()), fptrs(fused_ptrs.size());
+  for (size_t i = 0; i < ptrs.size(); ++i) ptrs[i] = reinterpret_cast<const void *>(layer_ptrs[i]);
+  for (size_t i = 0; i < fptrs.size(); ++i) fptrs[i] = reinterpret_cast<const void *>(fused_ptrs[i]);
+  a.fused_ptrs = fptrs.empty() ? nullptr : fptrs.data();
+  a.embed_weight = embed_weight.data_ptr();
+  a.layer_ptrs = ptrs.data();
+  a.final_norm_weight = final_norm_weight.data_ptr();
+  a.lm_head_weight = lm_head_weight.data_ptr();
+  a.cos_table = cos_table.data_ptr();
+  a.sin_table = sin_table.data_ptr();
+  a.num_seqs = c.cache.num_seqs;
+  a.num_layers = (int)num_layers;
+  a.max_seq_len = (int)max_seq_len;
+  a.attn_scale = (float)attn_scale;
+  a.num_rows = (int)R;
+  a.tokens = static_cast<const int *>(tokens.data_ptr());
+  a.row_seq = static_cast<const int *>(row_seq.data_ptr());
+  a.row_pos = static_cast<const int *>(row_pos.data_ptr());
+  a.num_out = (int)O;
+  a.workspace = workspace.data_ptr();
+  a.workspace_bytes = workspace.nbytes();
+  c10::cuda::CUDAGuard guard(embed_weight.device());
+  QmkBatchKvq kvq;
+  kvq.cache = c.cache;
+  kvq.code_layer_stride = k_codes.stride(1);
+  kvq.scale_layer_stride = k_scales.stride(1);
+  kvq.rows = c.rows;
+  const size_t need = qmk_kv_attend_workspace_bytes(&c.cache, &c.rows, QMK_NUM_Q_HEADS, QMK_FP16);
+  if (need == 0) raise_if_error(qmk_get_last_error());
+  torch::Tensor ws = torch::empty({(int64_t)need}, k_codes.options());
+  kvq.workspace = ws.data_ptr();
+  kvq.workspace_bytes = need;
+  kvq.status = c.status;
+  raise_if_error(qmk_batch_forward_kvq(&a, &kvq, c10::cuda::getCurrentCUDAStream().stream()));
+}
+
 int64_t workspace_bytes() { return (int64_t)qmk_workspace_bytes(); }
 
 void workspace_init(torch::Tensor workspace) {
@@ -730,6 +827,15 @@ TORCH_LIBRARY(qwen_megakernel_C, ops) {
   ops.def(("kv_attend(" + kv_cache_args + "Tensor q, Tensor out, " + kv_rows_args +
            ", float scale, Tensor? status) -> ()").c_str());
   ops.impl("kv_attend", torch::kCUDA, &kv_attend);
+
+  ops.def(("batch_forward_kvq(Tensor workspace, Tensor embed_weight, int[] layer_ptrs, int[] fused_ptrs, "
+           "Tensor final_norm_weight, Tensor lm_head_weight, Tensor cos_table, Tensor sin_table, "
+           "Tensor k_codes, Tensor v_codes, Tensor k_scales, Tensor v_scales, int bits, int max_seq_len, "
+           "float attn_scale, Tensor tokens, Tensor row_seq, Tensor row_pos, " +
+           std::string(kv_rows_args) +
+           ", Tensor? out_rows, Tensor? out_tokens, Tensor? logits, Tensor? status, Tensor? kv_status) -> ()")
+              .c_str());
+  ops.impl("batch_forward_kvq", torch::kCUDA, &batch_forward_kvq);
 
   ops.def("workspace_bytes() -> int", &workspace_bytes);
   ops.def("workspace_init(Tensor workspace) -> ()");

@@ -147,15 +147,19 @@ class QuantKVCache:
         for t in (self.k_codes, self.v_codes, self.k_scales, self.v_scales):
             t.zero_()
 
-    def _check(self, rows: KVRows, layer: int, *tensors) -> None:
-        if not 0 <= layer < self.num_layers:
-            raise ValueError(f"layer {layer} outside [0, {self.num_layers})")
+    def check_rows(self, rows: KVRows) -> None:
+        """Refuse what the host knows to be outside the cache."""
         if rows._num_seqs > self.num_seqs:
             raise ValueError(f"rows name sequence {rows._num_seqs - 1}; the cache has {self.num_seqs}")
         if rows._end > self.max_seq_len:
             raise ValueError(f"rows end at position {rows._end - 1}; max_seq_len is {self.max_seq_len}")
         if rows.max_rows > self.max_seq_len:
             raise ValueError(f"max_rows {rows.max_rows} exceeds max_seq_len {self.max_seq_len}")
+
+    def _check(self, rows: KVRows, layer: int, *tensors) -> None:
+        if not 0 <= layer < self.num_layers:
+            raise ValueError(f"layer {layer} outside [0, {self.num_layers})")
+        self.check_rows(rows)
         for name, t in tensors:
             if t.dim() != 3 or t.shape[0] != rows.rows or t.shape[2] != self.head_dim:
                 raise ValueError(f"{name} must be [rows={rows.rows}, heads, head_dim={self.head_dim}], "

@@ -220,3 +220,42 @@ def test_check_status_names_the_findings():
     with pytest.raises(KVCacheError, match="out of range.*NaN or infinity"):
         c.check_status()
     c.check_status()
+
+
+def test_batch_forward_kvq_refuses(lib):
+    """The forward pass over a quantized cache checks its arguments before it
+    touches a device."""
+    from test_batch_host import QmkBatchArgs
+
+    class Kvq(ctypes.Structure):
+        _fields_ = [("cache", Cache), ("code_layer_stride", i64), ("scale_layer_stride", i64), ("rows", Rows),
+                    ("workspace", vp), ("workspace_bytes", ctypes.c_size_t), ("status", vp)]
+
+    P = ctypes.POINTER
+    lib.qmk_batch_forward_kvq.argtypes = [P(QmkBatchArgs), P(Kvq), vp]
+    lib.qmk_batch_workspace_bytes.restype = ctypes.c_size_t
+    ptrs = (vp * 22)(*([FAKE] * 22))
+    rows = _rows()
+    need = lib.qmk_kv_attend_workspace_bytes(_cache(), rows, 16, 1)
+
+    def call(cache=None, rows=rows, code=8 * 256 * 64, scale=8 * 256 * 4, ws=FAKE, n=need, **kw):
+        f = dict(embed_weight=FAKE, layer_ptrs=ctypes.cast(ptrs, vp).value, final_norm_weight=FAKE,
+                 lm_head_weight=FAKE, cos_table=FAKE, sin_table=FAKE, num_seqs=2, num_layers=2, max_seq_len=200,
+                 num_rows=3, tokens=FAKE, row_seq=FAKE, row_pos=FAKE, workspace=FAKE, workspace_bytes=0)
+        f.update(kw)
+        return lib.qmk_batch_forward_kvq(QmkBatchArgs(**f), Kvq(cache or _cache(), code, scale, rows, ws, n, None),
+                                         None)
+
+    assert lib.qmk_batch_forward_kvq(QmkBatchArgs(), None, None) == QMK_ERR_ARGS
+    assert call() == QMK_ERR_WORKSPACE  # everything but the (empty) batch workspace is in order
+    assert b"qmk_batch_forward:" in lib.qmk_get_last_error_message()
+    for what in BAD_CACHES:
+        assert call(cache=_cache(**what)) == QMK_ERR_ARGS
+    for bad in (dict(cache=_cache(num_kv_heads=4)), dict(cache=_cache(head_dim=64)), dict(num_seqs=1),
+                dict(max_seq_len=199), dict(num_rows=4), dict(rows=_rows(segments=0, rows=3, row_offsets=FAKE)),
+                dict(rows=_rows(max_rows=0)), dict(code=1024), dict(scale=1024), dict(code=8 * 256 * 64 + 8),
+                dict(scale=8 * 256 * 4 + 4), dict(tokens=None), dict(num_layers=0)):
+        assert call(**bad) == QMK_ERR_ARGS, bad
+    for bad in (dict(ws=None), dict(n=need - 1), dict(ws=FAKE + 128)):
+        assert call(**bad) == QMK_ERR_WORKSPACE, bad
+        assert b"kvq" in lib.qmk_get_last_error_message()
