@@ -713,8 +713,10 @@ size_t workspace_need(const QmkKvCache *c, const QmkKvRows *r, int num_q_heads, 
   return kDescBytes + (parts + 255) / 256 * 256;
 }
 
+// Nothing is cut where no sequence can be longer than a tile.
 template <typename T, int D>
-cudaError_t launch_merge(const AttendArgs &a, int workers, int slots, int sms, cudaStream_t stream) {
+cudaError_t launch_merge(const AttendArgs &a, int tile, int workers, int slots, int sms, cudaStream_t stream) {
+  if (a.rows.max_seq_len <= tile) return cudaSuccess;
   int rb, hb, head_blocks;
   block_shape(slots, a.ratio, rb, hb, head_blocks);
   return launch_pdl(merge_kernel<T, D>, dim3(std::min(workers, 4 * sms), (slots + 15) / 16), 32 * kMergeWarps, 0,
@@ -735,7 +737,7 @@ int launch_attend(AttendArgs &a, int sms, int dev, cudaStream_t stream) {
     }
   }
   cudaError_t e = launch_pdl(attend_kernel<T, BITS, D, NT>, dim3(sms), 32 * S::kWarps, S::kSmem, stream, a);
-  if (e == cudaSuccess) e = launch_merge<T, D>(a, sms * S::kWarps, S::kSlots, sms, stream);
+  if (e == cudaSuccess) e = launch_merge<T, D>(a, S::kTile, sms * S::kWarps, S::kSlots, sms, stream);
   if (e != cudaSuccess) return fail(QMK_ERR_CUDA, "qmk_kv_attend launch: %s", cudaGetErrorString(e));
   return QMK_OK;
 }
@@ -744,8 +746,8 @@ template <typename T>
 int launch_tc_attend(const QmkKvCache *c, AttendArgs &a, int dtype, int sms, int dev, cudaStream_t stream) {
   cudaError_t e = attend_tc(a, dtype, c->bits, c->head_dim, sms, dev, stream);
   if (e == cudaSuccess)
-    e = c->head_dim == 128 ? launch_merge<T, 128>(a, sms, kTcLines, sms, stream)
-                           : launch_merge<T, 64>(a, sms, kTcLines, sms, stream);
+    e = c->head_dim == 128 ? launch_merge<T, 128>(a, 128, sms, kTcLines, sms, stream)
+                           : launch_merge<T, 64>(a, 128, sms, kTcLines, sms, stream);
   if (e != cudaSuccess) return fail(QMK_ERR_CUDA, "qmk_kv_attend launch: %s", cudaGetErrorString(e));
   return QMK_OK;
 }

@@ -600,41 +600,70 @@ void kv_write(torch::Tensor k_codes, torch::Tensor v_codes, torch::Tensor k_scal
   raise_if_error(qmk_kv_write(&c.cache, &c.rows, &kt, &vt, c.status, c10::cuda::getCurrentCUDAStream().stream()));
 }
 
-void kv_read(torch::Tensor k_codes, torch::Tensor v_codes, torch::Tensor k_scales, torch::Tensor v_scales,
-             int64_t bits, int64_t max_seq_len, int64_t layer, torch::Tensor k, torch::Tensor v, torch::Tensor start,
-             std::optional<torch::Tensor> row_offsets, std::optional<torch::Tensor> seq, int64_t max_rows,
-             std::optional<torch::Tensor> status) {
-  const KvCall c = kv_call(k_codes, v_codes, k_scales, v_scales, bits, max_seq_len, layer, k.dim() ? k.size(0) : 0,
-                           start, row_offsets, seq, max_rows, status);
+// Results of `rows` rows; cleared first where some row may belong to no segment.
+torch::Tensor kv_result(const torch::Tensor &like, int64_t rows, int64_t heads, int64_t head_dim,
+                        c10::ScalarType dtype, bool clear) {
+  const auto opt = like.options().dtype(dtype);
+  return clear ? torch::zeros({rows, heads, head_dim}, opt) : torch::empty({rows, heads, head_dim}, opt);
+}
+
+// Into k and v if given (and returns nothing), else into new tensors of `dtype`.
+std::tuple<torch::Tensor, torch::Tensor> kv_read(
+    torch::Tensor k_codes, torch::Tensor v_codes, torch::Tensor k_scales, torch::Tensor v_scales, int64_t bits,
+    int64_t max_seq_len, int64_t layer, std::optional<torch::Tensor> k_out, std::optional<torch::Tensor> v_out,
+    torch::Tensor start, std::optional<torch::Tensor> row_offsets, std::optional<torch::Tensor> seq, int64_t max_rows,
+    int64_t rows, c10::ScalarType dtype, bool clear, std::optional<torch::Tensor> status) {
+  QMK_CHECK(k_out.has_value() == v_out.has_value(), "k and v must be given together");
+  QMK_CHECK(rows >= 0, "rows must be >= 0");
+  const KvCall c = kv_call(k_codes, v_codes, k_scales, v_scales, bits, max_seq_len, layer, rows, start, row_offsets,
+                           seq, max_rows, status);
+  c10::cuda::CUDAGuard guard(k_codes.device());
+  torch::Tensor k, v;
+  if (k_out.has_value()) {
+    k = *k_out;
+    v = *v_out;
+  } else {
+    k = kv_result(k_codes, rows, c.cache.num_kv_heads, c.cache.head_dim, dtype, clear);
+    v = kv_result(k_codes, rows, c.cache.num_kv_heads, c.cache.head_dim, dtype, clear);
+  }
   const QmkKvTensor kt = kv_tensor(k, k_codes, "k", c.cache.num_kv_heads, c.cache.head_dim);
   const QmkKvTensor vt = kv_tensor(v, k_codes, "v", c.cache.num_kv_heads, c.cache.head_dim);
   check_writable(k, "k");
   check_writable(v, "v");
-  QMK_CHECK(v.size(0) == k.size(0) && v.scalar_type() == k.scalar_type(), "v must match k in rows and type");
-  if (k.size(0) == 0) return;
-  c10::cuda::CUDAGuard guard(k_codes.device());
-  raise_if_error(qmk_kv_read(&c.cache, &c.rows, &kt, &vt, c.status, c10::cuda::getCurrentCUDAStream().stream()));
+  QMK_CHECK(k.size(0) == rows && v.size(0) == rows && v.scalar_type() == k.scalar_type(),
+            "k and v must hold %lld rows of one type", (ll)rows);
+  if (rows > 0)
+    raise_if_error(qmk_kv_read(&c.cache, &c.rows, &kt, &vt, c.status, c10::cuda::getCurrentCUDAStream().stream()));
+  if (k_out.has_value()) return {torch::Tensor(), torch::Tensor()};
+  return {k, v};
 }
 
 // The workspace comes from the caching allocator on the current stream, so
 // calls on several streams and captured graphs never share one.
-void kv_attend(torch::Tensor k_codes, torch::Tensor v_codes, torch::Tensor k_scales, torch::Tensor v_scales,
-               int64_t bits, int64_t max_seq_len, int64_t layer, torch::Tensor q, torch::Tensor out,
-               torch::Tensor start, std::optional<torch::Tensor> row_offsets, std::optional<torch::Tensor> seq,
-               int64_t max_rows, double scale, std::optional<torch::Tensor> status) {
+// The result goes into out if given (and nothing is returned), else into a new tensor.
+torch::Tensor kv_attend(torch::Tensor k_codes, torch::Tensor v_codes, torch::Tensor k_scales, torch::Tensor v_scales,
+                        int64_t bits, int64_t max_seq_len, int64_t layer, torch::Tensor q,
+                        std::optional<torch::Tensor> out_given, torch::Tensor start,
+                        std::optional<torch::Tensor> row_offsets, std::optional<torch::Tensor> seq, int64_t max_rows,
+                        double scale, bool clear, std::optional<torch::Tensor> status) {
   const KvCall c = kv_call(k_codes, v_codes, k_scales, v_scales, bits, max_seq_len, layer, q.dim() ? q.size(0) : 0,
                            start, row_offsets, seq, max_rows, status);
   const QmkKvTensor qt = kv_tensor(q, k_codes, "q", -1, c.cache.head_dim);
+  c10::cuda::CUDAGuard guard(k_codes.device());
+  torch::Tensor out = out_given.has_value()
+                          ? *out_given
+                          : kv_result(k_codes, q.size(0), q.size(1), c.cache.head_dim, q.scalar_type(), clear);
   const QmkKvTensor ot = kv_tensor(out, k_codes, "out", q.size(1), c.cache.head_dim);
   check_writable(out, "out");
   QMK_CHECK(out.size(0) == q.size(0) && out.scalar_type() == q.scalar_type(), "out must match q in rows and type");
-  if (q.size(0) == 0) return;
-  c10::cuda::CUDAGuard guard(k_codes.device());
-  const size_t need = qmk_kv_attend_workspace_bytes(&c.cache, &c.rows, (int)q.size(1), qt.dtype);
-  if (need == 0) raise_if_error(qmk_get_last_error());
-  torch::Tensor ws = torch::empty({(int64_t)need}, k_codes.options());
-  raise_if_error(qmk_kv_attend(&c.cache, &c.rows, &qt, (int)q.size(1), &ot, (float)scale, ws.data_ptr(), need,
-                               c.status, c10::cuda::getCurrentCUDAStream().stream()));
+  if (q.size(0) > 0) {
+    const size_t need = qmk_kv_attend_workspace_bytes(&c.cache, &c.rows, (int)q.size(1), qt.dtype);
+    if (need == 0) raise_if_error(qmk_get_last_error());
+    torch::Tensor ws = torch::empty({(int64_t)need}, k_codes.options());
+    raise_if_error(qmk_kv_attend(&c.cache, &c.rows, &qt, (int)q.size(1), &ot, (float)scale, ws.data_ptr(), need,
+                                 c.status, c10::cuda::getCurrentCUDAStream().stream()));
+  }
+  return out_given.has_value() ? torch::Tensor() : out;
 }
 
 // The token-parallel forward pass over a quantized cache.
@@ -822,10 +851,13 @@ TORCH_LIBRARY(qwen_megakernel_C, ops) {
       "Tensor k_codes, Tensor v_codes, Tensor k_scales, Tensor v_scales, int bits, int max_seq_len, int layer, ";
   ops.def(("kv_write(" + kv_cache_args + "Tensor k, Tensor v, " + kv_rows_args + ", Tensor? status) -> ()").c_str());
   ops.impl("kv_write", torch::kCUDA, &kv_write);
-  ops.def(("kv_read(" + kv_cache_args + "Tensor k, Tensor v, " + kv_rows_args + ", Tensor? status) -> ()").c_str());
+  ops.def(("kv_read(" + kv_cache_args + "Tensor? k, Tensor? v, " + kv_rows_args +
+           ", int rows, ScalarType dtype, bool clear, Tensor? status) -> (Tensor, Tensor)")
+              .c_str());
   ops.impl("kv_read", torch::kCUDA, &kv_read);
-  ops.def(("kv_attend(" + kv_cache_args + "Tensor q, Tensor out, " + kv_rows_args +
-           ", float scale, Tensor? status) -> ()").c_str());
+  ops.def(("kv_attend(" + kv_cache_args + "Tensor q, Tensor? out, " + kv_rows_args +
+           ", float scale, bool clear, Tensor? status) -> Tensor")
+              .c_str());
   ops.impl("kv_attend", torch::kCUDA, &kv_attend);
 
   ops.def(("batch_forward_kvq(Tensor workspace, Tensor embed_weight, int[] layer_ptrs, int[] fused_ptrs, "

@@ -74,6 +74,7 @@ class KVRows:
             raise ValueError("too many rows")
         self.rows = offsets[-1]
         self.max_rows = max(counts_)
+        self._covers = True  # every row lies in a segment
         # host-known limits: checked against the cache at every call
         self._num_seqs = max(seqs) + 1
         self._end = max(s + c for s, c in zip(starts, counts_))
@@ -105,6 +106,7 @@ class KVRows:
             rows, max_rows = start.numel(), 1
         elif rows is None or max_rows is None:
             raise ValueError("row_offsets needs rows and max_rows")
+        self._covers = row_offsets is None
         self.rows, self.max_rows = int(rows), int(max_rows)
         if self.rows < 0 or self.max_rows < 0:
             raise ValueError("rows and max_rows must be >= 0")
@@ -125,7 +127,9 @@ class QuantKVCache:
             raise ValueError("head_dim must be 64 or 128")
         if min(num_seqs, max_seq_len, num_layers, num_kv_heads) < 1:
             raise ValueError("num_seqs, max_seq_len, num_layers and num_kv_heads must be >= 1")
-        self._ops = _native.ops()
+        ops = _native.ops()
+        # (the overloads themselves: looking them up costs a call about a microsecond)
+        self._write, self._read, self._attend = ops.kv_write.default, ops.kv_read.default, ops.kv_attend.default
         self.num_seqs, self.num_layers, self.num_kv_heads = int(num_seqs), int(num_layers), int(num_kv_heads)
         self.max_seq_len, self.head_dim, self.bits = int(max_seq_len), int(head_dim), int(bits)
         self.capacity = -(-self.max_seq_len // CAPACITY_STEP) * CAPACITY_STEP
@@ -136,6 +140,7 @@ class QuantKVCache:
         self.k_scales = torch.zeros(scales, dtype=torch.bfloat16, device=device)
         self.v_scales = torch.zeros_like(self.k_scales)
         self.device = self.k_codes.device
+        self._scale = 1.0 / math.sqrt(self.head_dim)
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
 
     @property
@@ -156,42 +161,40 @@ class QuantKVCache:
         if rows.max_rows > self.max_seq_len:
             raise ValueError(f"max_rows {rows.max_rows} exceeds max_seq_len {self.max_seq_len}")
 
-    def _check(self, rows: KVRows, layer: int, *tensors) -> None:
+    def _check(self, rows: KVRows, layer: int, name: str, t: torch.Tensor) -> None:
         if not 0 <= layer < self.num_layers:
             raise ValueError(f"layer {layer} outside [0, {self.num_layers})")
         self.check_rows(rows)
-        for name, t in tensors:
-            if t.dim() != 3 or t.shape[0] != rows.rows or t.shape[2] != self.head_dim:
-                raise ValueError(f"{name} must be [rows={rows.rows}, heads, head_dim={self.head_dim}], "
-                                 f"got {list(t.shape)}")
-
-    def _args(self, layer: int):
-        return (self.k_codes, self.v_codes, self.k_scales, self.v_scales, self.bits, self.max_seq_len, layer)
+        shape = t.shape
+        if len(shape) != 3 or shape[0] != rows.rows or shape[2] != self.head_dim:
+            raise ValueError(f"{name} must be [rows={rows.rows}, heads, head_dim={self.head_dim}], got {list(shape)}")
 
     def write(self, k: torch.Tensor, v: torch.Tensor, rows: KVRows, layer: int = 0) -> None:
         """Quantize ``k`` and ``v`` [rows, kv_heads, head_dim] (bf16, fp16 or
         fp32; any strides with head_dim contiguous) into the rows' positions.
         A NaN is held as 0 and an infinity as the group's end of range; either
         is reported by ``check_status``."""
-        self._check(rows, layer, ("k", k), ("v", v))
+        self._check(rows, layer, "k", k)  # (v must match k: the operator checks it)
         if rows._overlap:
             raise ValueError("rows hold a position of a sequence twice")
-        self._ops.kv_write(*self._args(layer), k, v, rows.start, rows.row_offsets, rows.seq, rows.max_rows,
-                           self.status)
+        self._write(self.k_codes, self.v_codes, self.k_scales, self.v_scales, self.bits, self.max_seq_len, layer, k, v,
+                    rows.start, rows.row_offsets, rows.seq, rows.max_rows, self.status)
 
     def read(self, rows: KVRows, layer: int = 0, dtype: torch.dtype = torch.bfloat16,
              out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
         """The values that the rows' positions hold, (k, v) [rows, kv_heads,
         head_dim], rounded to ``dtype``; into ``out`` (and its type) if given."""
-        if out is None:
-            shape = (rows.rows, self.num_kv_heads, self.head_dim)
-            # rows that no segment holds are not written: never hand out what was in memory before
-            make = torch.empty if rows._num_seqs else torch.zeros
-            out = (make(shape, dtype=dtype, device=self.device), make(shape, dtype=dtype, device=self.device))
-        self._check(rows, layer, ("out[0]", out[0]), ("out[1]", out[1]))
-        self._ops.kv_read(*self._args(layer), out[0], out[1], rows.start, rows.row_offsets, rows.seq, rows.max_rows,
-                          self.status)
-        return out
+        k, v = (None, None) if out is None else out
+        if out is not None:
+            self._check(rows, layer, "out[0]", k)
+        elif not 0 <= layer < self.num_layers:
+            raise ValueError(f"layer {layer} outside [0, {self.num_layers})")
+        else:
+            self.check_rows(rows)
+        new = self._read(self.k_codes, self.v_codes, self.k_scales, self.v_scales, self.bits, self.max_seq_len, layer,
+                         k, v, rows.start, rows.row_offsets, rows.seq, rows.max_rows, rows.rows, dtype,
+                         not rows._covers, self.status)
+        return new if out is None else out
 
     def attend(self, q: torch.Tensor, rows: KVRows, layer: int = 0, scale: float | None = None,
                out: torch.Tensor | None = None) -> torch.Tensor:
@@ -200,17 +203,16 @@ class QuantKVCache:
         head j to K/V head ``j // (q_heads / kv_heads)``.  ``scale`` defaults to
         1 / sqrt(head_dim).  Returns ``out`` (q's type and shape); rows that no
         segment holds are left as they are in a given ``out`` and 0 else."""
-        self._check(rows, layer, ("q", q))
-        if q.shape[1] < 1 or q.shape[1] % self.num_kv_heads or q.shape[1] // self.num_kv_heads > MAX_RATIO:
-            raise ValueError(f"q has {q.shape[1]} heads: not 1 .. {MAX_RATIO} times the cache's {self.num_kv_heads}")
-        if out is None:
-            make = torch.empty if rows._num_seqs else torch.zeros
-            out = make(q.shape, dtype=q.dtype, device=q.device)
-        elif out.shape != q.shape or out.dtype != q.dtype:
+        self._check(rows, layer, "q", q)
+        heads = q.shape[1]
+        if heads < 1 or heads % self.num_kv_heads or heads // self.num_kv_heads > MAX_RATIO:
+            raise ValueError(f"q has {heads} heads: not 1 .. {MAX_RATIO} times the cache's {self.num_kv_heads}")
+        if out is not None and (out.shape != q.shape or out.dtype != q.dtype):
             raise ValueError("out must have q's shape and type")
-        self._ops.kv_attend(*self._args(layer), q, out, rows.start, rows.row_offsets, rows.seq, rows.max_rows,
-                            1.0 / math.sqrt(self.head_dim) if scale is None else float(scale), self.status)
-        return out
+        new = self._attend(self.k_codes, self.v_codes, self.k_scales, self.v_scales, self.bits, self.max_seq_len,
+                           layer, q, out, rows.start, rows.row_offsets, rows.seq, rows.max_rows,
+                           self._scale if scale is None else float(scale), not rows._covers, self.status)
+        return new if out is None else out
 
     def check_status(self) -> None:
         """Raise KVCacheError if a call since the last check reported
