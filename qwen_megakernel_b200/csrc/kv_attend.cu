@@ -535,32 +535,41 @@ __global__ void __launch_bounds__(32 * Shape<T, BITS, D, NT>::kWarps, 1)
   }
 }
 
-// Joins the parts of items that were cut: CTA c takes the items whose first
-// tile is in the range of worker c, c + grid, ... and that go on in the next
-// ranges.  A warp takes an output row, or several share one (few rows mean
-// many parts); 8 parts are loaded at a time.  Grid y shares an item's rows.
-constexpr int kMergeWarps = 8;
+// Joins the parts of items that were cut: CTA x takes the items whose first
+// tile is in the range of one of its workers and that go on in the next
+// ranges, grid y shares their rows.  A warp takes an output row, or several
+// share one (few rows mean many parts, 222 a row for one stream of 32k);
+// kMergeBatch parts are loaded at a time.  What it takes is latency: of the
+// descriptor, of a round of parts, of the warps' sums.
+constexpr int kMergeWarps = 8, kMergeBatch = 4;
 
 template <typename T, int D>
-__global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const int *__restrict__ desc,
-                                                                 const float *__restrict__ parts, int workers,
-                                                                 int slots, int hb, void *out, long long o_row,
-                                                                 long long o_head) {
-  pdl_wait();  // the parts are written by attend_kernel
+__global__ void __launch_bounds__(32 * kMergeWarps, 4) merge_kernel(const int *__restrict__ desc,
+                                                                    const float *__restrict__ parts, int workers,
+                                                                    int slots, void *out, long long o_row,
+                                                                    long long o_head) {
+  pdl_wait();  // the parts are written by the attention kernel
   pdl_trigger();
   __shared__ float s_ml[kMergeWarps][2];
   __shared__ float s_o[kMergeWarps][D];
   constexpr int kPer = D / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int c = blockIdx.x; c < workers; c += gridDim.x) {
+  // the CTA's workers, a lane each (the host keeps them to 32); neighbours, for
+  // heads of long items lie a regular distance apart
+  const int per = (workers + gridDim.x - 1) / gridDim.x, mine = blockIdx.x * per + lane;
+  const int np_mine = lane < per && mine < workers ? __ldcg(desc + (size_t)mine * kDescWords) : 0;
+  for (unsigned todo = __ballot_sync(0xffffffffu, np_mine > 0); todo; todo &= todo - 1) {
+    const int src = __ffs(todo) - 1, c = blockIdx.x * per + src;
+    const int np = __shfl_sync(0xffffffffu, np_mine, src);
     const int *dd = desc + (size_t)c * kDescWords;
-    const int np = dd[0];
-    if (np == 0) continue;
-    const int row0 = dd[1], nrows = dd[2], head0 = dd[3], nheads = dd[4], n = nrows * nheads;
-    const int share = n >= kMergeWarps ? 1 : kMergeWarps / n, at_once = kMergeWarps / share;  // warps a row, rows
-    for (int v0 = blockIdx.y * at_once; v0 < n; v0 += gridDim.y * at_once) {
+    const int4 d4 = __ldcg(reinterpret_cast<const int4 *>(dd + 4));
+    const int row0 = d4.x, nrows = d4.y, head0 = d4.z, nheads = d4.w & 0xffff, hb = d4.w >> 16, n = nrows * nheads;
+    // rows [v_lo, v_hi) of this CTA; `share` warps a row
+    const int each = (n + gridDim.y - 1) / gridDim.y, v_lo = blockIdx.y * each, v_hi = min(n, v_lo + each);
+    const int share = each >= kMergeWarps ? 1 : kMergeWarps / each, at_once = kMergeWarps / share;
+    for (int v0 = v_lo; v0 < v_hi; v0 += at_once) {
       const int v = v0 + warp / share, first = warp % share;
-      const bool live = v < n && warp < share * at_once;
+      const bool live = v < v_hi && warp < share * at_once;
       const int i = live ? v / nheads : 0, j = live ? v % nheads : 0;
       // part k: worker c + k's, the head part first
       const float *p0 = parts + ((size_t)c * 2 * slots + i * hb + j) * (D + 4) + kPer * lane;
@@ -568,14 +577,13 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const int *__re
       float M = -INFINITY, L = 0.f, y[kPer];
 #pragma unroll
       for (int e = 0; e < kPer; ++e) y[e] = 0.f;
-      for (int k0 = first; live && k0 < np; k0 += 8 * share) {
-        float2 ml[8];
-        float x[8][kPer];
+      for (int k0 = first; live && k0 < np; k0 += kMergeBatch * share) {
+        float2 ml[kMergeBatch];
+        float x[kMergeBatch][kPer];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const int k = k0 + q * share;
-          ml[q] = make_float2(-INFINITY, 0.f);
-          if (k >= np) continue;
+        for (int q = 0; q < kMergeBatch; ++q) {
+          // (the last part again rather than a branch round each load)
+          const int k = min(k0 + q * share, np - 1);
           const float *p = p0 + k * step + (k == 0 ? 0 : tail);
           ml[q] = __ldcg(reinterpret_cast<const float2 *>(p - kPer * lane + D));
           if constexpr (kPer == 4) *reinterpret_cast<float4 *>(x[q]) = __ldcg(reinterpret_cast<const float4 *>(p));
@@ -583,16 +591,16 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const int *__re
         }
         float mn = M;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) mn = fmaxf(mn, ml[q].x);
+        for (int q = 0; q < kMergeBatch; ++q) mn = fmaxf(mn, ml[q].x);
         const float ref = mn == -INFINITY ? 0.f : mn, corr = fast_exp2(M - ref);
         M = mn;
         L *= corr;
 #pragma unroll
         for (int e = 0; e < kPer; ++e) y[e] *= corr;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          if (k0 + q * share >= np) continue;
-          const float w = fast_exp2(ml[q].x - ref);  // (0 times a NaN state: NaN)
+        for (int q = 0; q < kMergeBatch; ++q) {
+          // (0 times a NaN state: NaN)
+          const float w = fast_exp2(ml[q].x - ref) * (k0 + q * share < np ? 1.f : 0.f);
           L = fmaf(w, ml[q].y, L);
 #pragma unroll
           for (int e = 0; e < kPer; ++e) y[e] = fmaf(w, x[q][e], y[e]);
@@ -717,10 +725,9 @@ size_t workspace_need(const QmkKvCache *c, const QmkKvRows *r, int num_q_heads, 
 template <typename T, int D>
 cudaError_t launch_merge(const AttendArgs &a, int tile, int workers, int slots, int sms, cudaStream_t stream) {
   if (a.rows.max_seq_len <= tile) return cudaSuccess;
-  int rb, hb, head_blocks;
-  block_shape(slots, a.ratio, rb, hb, head_blocks);
-  return launch_pdl(merge_kernel<T, D>, dim3(std::min(workers, 4 * sms), (slots + 15) / 16), 32 * kMergeWarps, 0,
-                    stream, (const int *)a.desc, (const float *)a.parts, workers, slots, hb, a.out, a.o_row, a.o_head);
+  const int grid = std::max((workers + 31) / 32, std::min(workers, 3 * sms));
+  return launch_pdl(merge_kernel<T, D>, dim3(grid, slots > 16 ? 16 : 2), 32 * kMergeWarps, 0, stream,
+                    (const int *)a.desc, (const float *)a.parts, workers, slots, a.out, a.o_row, a.o_head);
 }
 
 template <typename T, int BITS, int D, int NT>

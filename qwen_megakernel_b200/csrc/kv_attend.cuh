@@ -210,12 +210,12 @@ __device__ inline Item next_item(const Rows &R, Range &r, Segment &s, int rb, in
 // Tells merge_kernel about an item whose head part worker `me` holds.
 __device__ __forceinline__ void describe_cut(int *desc, const Item &it, const Segment &s, const Range &r, long long me,
                                              int ratio, int hb) {
-  desc[1] = s.r0 + it.row0;
-  desc[2] = it.nrows;
-  desc[3] = it.h * ratio + it.head0;
-  desc[4] = min(hb, ratio - it.head0);
   // parts: this worker's and those up to the worker with the item's last tile
   desc[0] = (int)(quotient((it.u0 + it.tiles) * r.workers - 1, r.total) - me) + 1;
+  desc[4] = s.r0 + it.row0;
+  desc[5] = it.nrows;
+  desc[6] = it.h * ratio + it.head0;
+  desc[7] = min(hb, ratio - it.head0) | hb << 16;
 }
 
 // ------------------------------------------------------------- instructions
