@@ -417,33 +417,61 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
         const int pos0 = (it.t_lo + i) * kPos;
         if (!wait_warp(&B.s_full[x], n_s & 1, abort)) return false;
         tc_fence_after_sync();
-        const float ck = cm * B.exp_k[g & 3], ev = B.exp_v[g & 3];
+        const float ck = fmaxf(cm * B.exp_k[g & 3], 1.2e-38f), ev = B.exp_v[g & 3];  // (> 0: -inf stays -inf)
         const bool all = pos0 + kPos <= it.seen_by_all();
-        float mx = -INFINITY;
-#pragma unroll 1
-        for (int c = 0; c < kPos; c += 64) {
-          uint32_t r0[32], r1[32];
-          tmem_ld32_async(s_at + c, r0);
-          tmem_ld32_async(s_at + c + 32, r1);
-          tmem_ld_wait(r0);
-          tmem_ld_wait(r1);
-          if (!all) {
+        float mx, f = 1.f, sum0, sum1;
+        uint32_t p[kPos / 2];
+        // One pass over S: P against the reference R, kept in registers so that
+        // S stays until R is known to do, and the maximum on the way.
+        auto pass = [&](auto masked) {
+          const float add = ev + kTcShift - (R == -INFINITY ? 0.f : R);
+          mx = -INFINITY;
+          sum0 = sum1 = 0.f;
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              if (pos0 + c + e >= lim) r0[e] = 0xff800000u;  // -inf
-              if (pos0 + c + 32 + e >= lim) r1[e] = 0xff800000u;
+          for (int c = 0; c < kPos; c += 32) {
+            uint32_t r[32];
+            tmem_ld32_async(s_at + c, r);
+            tmem_ld_wait(r);
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              if constexpr (decltype(masked)::value) {
+                if (pos0 + c + e >= lim) r[e] = 0xff800000u;  // -inf
+                if (pos0 + c + e + 1 >= lim) r[e + 1] = 0xff800000u;
+              }
+              float y0 = __uint_as_float(r[e]), y1 = __uint_as_float(r[e + 1]);
+              mx = fmaxf(mx, fmaxf(y0, y1));
+              fma2(y0, y1, ck, add);
+              y0 = fast_exp2(y0);
+              y1 = fast_exp2(y1);
+              add2(sum0, sum1, y0, y1);
+              p[(c + e) / 2] = pack_f16(y0, y1);
             }
           }
+        };
+        if (i == 0) {  // the first maximum by itself
+          float m0 = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; c < kPos; c += 32) {
+            uint32_t r[32];
+            tmem_ld32_async(s_at + c, r);
+            tmem_ld_wait(r);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) mx = fmaxf(mx, fmaxf(__uint_as_float(r0[e]), __uint_as_float(r1[e])));
+            for (int e = 0; e < 32; ++e) m0 = fmaxf(m0, pos0 + c + e < lim ? __uint_as_float(r[e]) : -INFINITY);
+          }
+          R = fmaf(m0, ck, ev);
         }
-        const float m = fmaf(mx, ck, ev);  // of score + E
-        float f = 1.f;
-        if (m > R + kTcSlack) {  // (R = -inf at first)
-          f = fast_exp2(R - m);
-          R = m;
-        }
-        if (i > 0 && __any_sync(0xffffffffu, f != 1.f)) {
+#pragma unroll 1
+        for (;;) {
+          if (all) pass(std::false_type{});
+          else pass(std::true_type{});
+          const float m = fmaf(mx, ck, ev);  // of score + E
+          const bool behind = m > R + kTcSlack;
+          if (!__any_sync(0xffffffffu, behind)) break;
+          // rare: the reference moves, O with it (i > 0: at i = 0 R is the maximum)
+          if (behind) {
+            f = fast_exp2(R - m);
+            R = m;
+          }
           if (!wait_warp(&B.pv[x], (n_s - 1) & 1, abort)) return false;
           tc_fence_after_sync();
 #pragma unroll 1
@@ -455,41 +483,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
             tmem_st16(o_at + c, r);
           }
         }
-        const float add = ev + kTcShift - (R == -INFINITY ? 0.f : R);
-        float sum0 = 0.f, sum1 = 0.f;
-        // 32 columns: P's first columns replace S's, behind what has been read
-        auto exps = [&](uint32_t(&v)[32], int c, auto masked) {
-          uint32_t p[16];
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            float y0 = __uint_as_float(v[e]), y1 = __uint_as_float(v[e + 1]);
-            fma2(y0, y1, ck, add);
-            y0 = fast_exp2(y0);
-            y1 = fast_exp2(y1);
-            if constexpr (decltype(masked)::value) {
-              y0 = pos0 + c + e < lim ? y0 : 0.f;
-              y1 = pos0 + c + e + 1 < lim ? y1 : 0.f;
-            }
-            add2(sum0, sum1, y0, y1);
-            p[e / 2] = pack_f16(y0, y1);
-          }
-          tmem_st16(s_at + c / 2, p);
-        };
-        auto pass = [&](auto masked) {
-          uint32_t r0[32], r1[32];
-          tmem_ld32_async(s_at, r0);
-#pragma unroll 1
-          for (int c = 0; c < kPos; c += 64) {
-            tmem_ld_wait(r0);
-            tmem_ld32_async(s_at + c + 32, r1);
-            exps(r0, c, masked);
-            tmem_ld_wait(r1);
-            if (c + 64 < kPos) tmem_ld32_async(s_at + c + 64, r0);
-            exps(r1, c + 32, masked);
-          }
-        };
-        if (all) pass(std::false_type{});
-        else pass(std::true_type{});
+        for (int c = 0; c < kPos / 2; c += 16) {  // over S's first columns
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) w[e] = p[c + e];
+          tmem_st16(s_at + c, w);
+        }
         tmem_st_wait();
         tc_fence_before_sync();
         __syncwarp();
