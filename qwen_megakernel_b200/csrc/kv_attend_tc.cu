@@ -56,9 +56,13 @@ struct TcShape {
   static constexpr int kCodeBytes = kPos * kRowBytes;
   static constexpr int kScaleBytes = kPos * kGroups * 2;
   static constexpr int kRawBytes = kCodeBytes + kScaleBytes;           // of K or V
-  static constexpr int kRawSlots = kRowBytes == 128 ? 3 : 4;           // K, V, K, V, ... take turns
+  static constexpr int kRawSlots = 3;                                  // K, V, K, V, ... take turns
+  // Two places of decoded K where they fit (8 bits x 128: 34 KB of raw slots
+  // more): with one, decoding waits for B's scores and A's next for decoding
+  // (a tile 6.4k cycles).
+  static constexpr int kKBufs = kRowBytes == 128 ? 1 : 2;
   static constexpr int kTileBytes = kPos * D * 2;                      // fp16, two halves of 64 dimensions (one)
-  static constexpr int kQ = 0, kK = kLines * D * 2, kV = kK + kTileBytes, kRaw = kV + 2 * kTileBytes;
+  static constexpr int kQ = 0, kK = kLines * D * 2, kV = kK + kKBufs * kTileBytes, kRaw = kV + 2 * kTileBytes;
   static constexpr int kRawSlot = (kRawBytes + 1023) / 1024 * 1024;
   static constexpr int kBars = kRaw + kRawSlots * kRawSlot;
   static constexpr int kSmem = 1024 + kBars + 512;
@@ -67,7 +71,7 @@ struct TcShape {
 
 struct TcBars {
   uint64_t raw_full[4], raw_empty[4];
-  uint64_t k_full, k_empty, v_full[2], v_empty[2];  // decoded tiles; empty: read by the MMAs
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];  // decoded tiles; empty: read by the MMAs
   uint64_t s_full[2], p_full[2], pv[2];             // of A and B; pv: P V of a tile done
   uint64_t q_full, drain;
   float exp_k[4], exp_v[4];  // 2^E of K and E of V, of tile t in slot t % 4
@@ -76,15 +80,59 @@ struct TcBars {
 };
 static_assert(sizeof(TcBars) <= 512, "barrier area");
 
-__device__ __forceinline__ void mma_ts_warp(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+// The K steps of a tile's product, issued by one elected lane of a converged
+// warp in one go (an election an MMA cost 70 cycles each, the issuer was what
+// the softmax waited for).  Descriptors advance by 16-byte units: 32 bytes a
+// step within 64 dimensions of Q and K, 16 positions (2048 bytes) of V; P by 8
+// TMEM columns.
+#define QKV_MMA(A, AS, B, BS) "@e tcgen05.mma.cta_group::1.kind::f16 [%0], " A ", b, %3, p;\n\t" AS BS
+template <int STEPS>
+__device__ __forceinline__ void mma_scores(uint32_t d, uint64_t q, uint64_t k, uint32_t idesc) {
+  static_assert(STEPS == 4 || STEPS == 8, "64 or 128 dimensions");
   asm volatile(
-      "{\n\t.reg .pred p, e;\n\t"
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 a, b;\n\t"
       "elect.sync _|e, 0xffffffff;\n\t"
+      "mov.b64 a, %1;\n\tmov.b64 b, %2;\n\t"
+      "setp.ne.b32 p, 0, 0;\n\t"
+      QKV_MMA("a", "add.s64 a, a, 2;\n\t", "b", "add.s64 b, b, 2;\n\t")
+      "setp.eq.b32 p, 0, 0;\n\t"
+      QKV_MMA("a", "add.s64 a, a, 2;\n\t", "b", "add.s64 b, b, 2;\n\t")
+      QKV_MMA("a", "add.s64 a, a, 2;\n\t", "b", "add.s64 b, b, 2;\n\t")
+      QKV_MMA("a", "", "b", "")
+      "}" ::"r"(d), "l"(q), "l"(k), "r"(idesc)
+      : "memory");
+  if constexpr (STEPS == 8)  // the second 64 dimensions
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t.reg .b64 a, b;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "mov.b64 a, %1;\n\tmov.b64 b, %2;\n\t"
+        "setp.eq.b32 p, 0, 0;\n\t"
+        QKV_MMA("a", "add.s64 a, a, 2;\n\t", "b", "add.s64 b, b, 2;\n\t")
+        QKV_MMA("a", "add.s64 a, a, 2;\n\t", "b", "add.s64 b, b, 2;\n\t")
+        QKV_MMA("a", "add.s64 a, a, 2;\n\t", "b", "add.s64 b, b, 2;\n\t")
+        QKV_MMA("a", "", "b", "")
+        "}" ::"r"(d), "l"(q + (kHalf * 128 >> 4)), "l"(k + (kPos * 128 >> 4)), "r"(idesc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_outputs(uint32_t d, uint32_t p_cols, uint64_t v, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t.reg .b32 a;\n\t.reg .b64 b;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "mov.b32 a, %1;\n\tmov.b64 b, %2;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+      QKV_MMA("[a]", "add.s32 a, a, 8;\n\t", "b", "add.s64 b, b, 128;\n\t")
+      "setp.eq.b32 p, 0, 0;\n\t"
+      QKV_MMA("[a]", "add.s32 a, a, 8;\n\t", "b", "add.s64 b, b, 128;\n\t")
+      QKV_MMA("[a]", "add.s32 a, a, 8;\n\t", "b", "add.s64 b, b, 128;\n\t")
+      QKV_MMA("[a]", "add.s32 a, a, 8;\n\t", "b", "add.s64 b, b, 128;\n\t")
+      QKV_MMA("[a]", "add.s32 a, a, 8;\n\t", "b", "add.s64 b, b, 128;\n\t")
+      QKV_MMA("[a]", "add.s32 a, a, 8;\n\t", "b", "add.s64 b, b, 128;\n\t")
+      QKV_MMA("[a]", "add.s32 a, a, 8;\n\t", "b", "add.s64 b, b, 128;\n\t")
+      QKV_MMA("[a]", "", "b", "")
+      "}" ::"r"(d), "r"(p_cols), "l"(v), "r"(idesc), "r"((uint32_t)accumulate)
       : "memory");
 }
+#undef QKV_MMA
 // TMEM loads that are waited for apart (tmem_ld_wait), so that one can be in
 // flight while the last one's values are used.
 __device__ __forceinline__ void tmem_ld32_async(uint32_t taddr, uint32_t (&r)[32]) {
@@ -199,7 +247,7 @@ __host__ __device__ constexpr int order(int slot) {
 template <typename T, int BITS, int D>
 __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_constant__ AttendArgs a) {
   using S = TcShape<BITS, D>;
-  constexpr int G = S::kGroups, RS = S::kRawSlots;
+  constexpr int G = S::kGroups, RS = S::kRawSlots, KB = S::kKBufs;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   TcBars &B = *reinterpret_cast<TcBars *>(smem + S::kBars);
@@ -210,9 +258,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
       mbar_init(&B.raw_full[i], 1);
       mbar_init(&B.raw_empty[i], 4);
     }
-    mbar_init(&B.k_full, 4);
-    mbar_init(&B.k_empty, 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&B.k_full[i], 4);
+      mbar_init(&B.k_empty[i], 1);
       mbar_init(&B.v_full[i], 4);
       mbar_init(&B.v_empty[i], 1);
       mbar_init(&B.s_full[i], 2);  // the MMAs' commit, and the issuer itself: it passes the exponents on
@@ -292,18 +340,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
     constexpr uint32_t kIdesc = (1u << 4) | ((uint32_t)(kHalf >> 4) << 24);  // fp16 x fp16 -> fp32, M = 128
     constexpr uint32_t kIdescS = kIdesc | ((uint32_t)(kPos >> 3) << 17);
     constexpr uint32_t kIdescO = kIdesc | (1u << 16) | ((uint32_t)(D >> 3) << 17);  // V: MN-major
-    const uint32_t k0 = smem_addr(smem + S::kK);
     // S of line tile x (MMAs run in the order of issue: what P V of the tile before reads of P comes first)
-    auto scores = [&](int x, bool last) {
+    auto scores = [&](int x, unsigned g, bool last) {
+      const uint32_t k0 = smem_addr(smem + S::kK + (g % KB) * S::kTileBytes);
       const uint32_t q0 = smem_addr(smem + S::kQ) + x * (kHalf * D * 2);
-#pragma unroll
-      for (int s = 0; s < D / 16; ++s) {
-        const uint32_t half = (s / 4) * (kPos * 128), in = (s % 4) * 32;
-        tc_mma_bf16_warp(tmem + kColS + 128 * x, smem_desc_sw128(q0 + half + in, 1024u),
-                         smem_desc_sw128(k0 + half + in, 1024u), kIdescS, s > 0);
-      }
+      mma_scores<D / 16>(tmem + kColS + 128 * x, smem_desc_sw128(q0, 1024u), smem_desc_sw128(k0, 1024u), kIdescS);
       tc_commit_warp(&B.s_full[x]);
-      if (last) tc_commit_warp(&B.k_empty);
+      if (last) tc_commit_warp(&B.k_empty[g % KB]);
       if (lane == 0) mbar_arrive(&B.s_full[x]);
     };
     unsigned n_p[2] = {0, 0};
@@ -311,17 +354,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
       if (!wait_warp(&B.p_full[x], n_p[x]++ & 1, abort)) return false;
       tc_fence_after_sync();
       const uint32_t v0 = smem_addr(smem + S::kV + (g & 1) * S::kTileBytes);
-#pragma unroll
-      for (int s = 0; s < kPos / 16; ++s)
-        mma_ts_warp(tmem + kColO + 128 * x, tmem + kColS + 128 * x + 8 * s, desc_mn(v0 + s * 2048, kPos * 128), kIdescO,
-                    !first || s > 0);
+      static_assert(kPos == 128, "8 steps");
+      mma_outputs(tmem + kColO + 128 * x, tmem + kColS + 128 * x, desc_mn(v0, kPos * 128), kIdescO, !first);
       tc_commit_warp(&B.pv[x]);
       if (last) tc_commit_warp(&B.v_empty[g & 1]);
       return true;
     };
     // K and V of tile g decoded: V too, since the scores' barrier passes both exponents on
     auto tiles_ready = [&](unsigned g) {
-      if (!wait_warp(&B.k_full, g & 1, abort)) return false;
+      if (!wait_warp(&B.k_full[g % KB], (g / KB) & 1, abort)) return false;
       if (!wait_warp(&B.v_full[g & 1], (g >> 1) & 1, abort)) return false;
       tc_fence_after_sync();
       return true;
@@ -332,19 +373,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
       const bool two = it.nrows * hb > kHalf;
       if (!wait_warp(&B.q_full, item++ & 1, abort)) return false;
       if (!tiles_ready(t)) return false;
-      scores(0, !two);
-      if (two) scores(1, true);
+      scores(0, t, !two);
+      if (two) scores(1, t, true);
       for (int i = 0; i < nt; ++i) {
         const unsigned g = t + i;
         const bool more = i + 1 < nt;
+        // (decoded long before A's P as a rule: waited for here, off A's way)
+        if (more && !tiles_ready(g + 1)) return false;
         if (!outputs(0, g, i == 0, !two)) return false;
-        if (more) {
-          if (!tiles_ready(g + 1)) return false;
-          scores(0, !two);
-        }
+        if (more) scores(0, g + 1, !two);
         if (two) {
           if (!outputs(1, g, i == 0, true)) return false;
-          if (more) scores(1, true);
+          if (more) scores(1, g + 1, true);
         }
       }
       t += nt;
@@ -612,15 +652,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
 #pragma unroll
           for (int k = 0; k < G; ++k) sc[k] = pack_f16(s[k] * down, s[k] * down);
         }
-        // the tile's place has been read: K's by the scores of g - 1, V's by the outputs of g - 2
+        // the tile's place has been read: K's by the scores of g - KB, V's by the outputs of g - 2
         if (side ? g >= 2 && !wait_warp(&B.v_empty[b], ((g >> 1) - 1) & 1, abort)
-                 : g >= 1 && !wait_warp(&B.k_empty, (g - 1) & 1, abort))
+                 : g >= KB && !wait_warp(&B.k_empty[g % KB], (g / KB - 1) & 1, abort))
           return false;
-        uint8_t *tile = smem + (side ? S::kV + b * S::kTileBytes : S::kK);
+        uint8_t *tile = smem + (side ? S::kV + b * S::kTileBytes : S::kK + (g % KB) * S::kTileBytes);
         constexpr int kPerLine = 128 / S::kRowBytes;
         const uint8_t *src = raw + (p / kPerLine) * 128;
         const int src_swz = (p / kPerLine) & 7;
-#pragma unroll 1
+#pragma unroll
         for (int c = 0; c < S::kRowBytes / 16; ++c) {
           const uint4 w = *reinterpret_cast<const uint4 *>(
               src + ((((p % kPerLine) * (S::kRowBytes / 16) + c) ^ src_swz) << 4));
@@ -629,9 +669,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
 #pragma unroll
           for (int k = 0; k < kOut; ++k) {
             const int oc = c * kOut + k;  // dimensions 8 oc ..
-            unsigned s2 = sc[0];
-#pragma unroll
-            for (int q = 1; q < G; ++q) s2 = oc / 4 == q ? sc[q] : s2;
+            const unsigned s2 = sc[oc / 4];
             unsigned h[4];
             if constexpr (BITS == 4) {
               dec.nibbles(ww[k], h);
@@ -653,7 +691,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
           if (warp == 12) B.exp_k[g & 3] = __uint_as_float((unsigned)e << 23);
           if (warp == 16) B.exp_v[g & 3] = (float)(e - 127);
           mbar_arrive(&B.raw_empty[st]);
-          mbar_arrive(side ? &B.v_full[b] : &B.k_full);
+          mbar_arrive(side ? &B.v_full[b] : &B.k_full[g % KB]);
         }
       }
       t += nt;
