@@ -28,13 +28,11 @@
 
 #include "kv_attend.cuh"
 
-int qmk_internal_set_error(int code, const char *msg);
 int qmk_internal_clear_error();
 
 namespace qkv {
 
 constexpr float kLog2e = 1.4426950408889634f;
-
 
 // ------------------------------------------------------------- instructions
 __device__ __forceinline__ void mma_f16(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
@@ -66,6 +64,7 @@ __device__ __forceinline__ unsigned transpose8(unsigned x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
+
 __device__ __forceinline__ bool wait_copy(uint64_t *bar, unsigned parity) {
   uint64_t t0 = 0;
   for (unsigned it = 0;; ++it) {
@@ -691,14 +690,21 @@ cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, int block, size_t sm
 }
 
 // Slots an item holds: one N = 8 tile, or two where the segments' rows and
-// heads fill more than one.
+// heads fill more than two (an item of two decodes the cache once for both, but
+// its warps need 255 registers, 8 to an SM).  Measured, us with one / two tiles
+// an item, 4 bits x 128, 2 q heads a K/V head, 4000 positions:
+//   1 sequence    10 columns 18.3 / 25.6   16: 19.0 / 26.0   32: 24.1 / 27.7
+//   16 sequences  10 columns 45.1 / 44.3   16: 46.0 / 46.1   32: 81.5 / 69.8
 int tiles_n(int dtype, int max_rows, int ratio) {
-  return (long long)max_rows * ratio > (dtype == QMK_FP32 ? 4 : 8) ? 2 : 1;
+  return (long long)max_rows * ratio > (dtype == QMK_FP32 ? 8 : 16) ? 2 : 1;
 }
 int slots_of(int dtype, int nt) { return nt * (dtype == QMK_FP32 ? 4 : 8); }
 
-// Where the tcgen05 kernel takes over: its 128 query lines cost the same
-// however few are used.
+// Where the tcgen05 kernel takes over: its lines come in 128s and cost the same
+// however few are used, the warps' kernel decodes the cache again for every 16
+// columns.  Measured as above, us of the warps' / the tcgen05 kernel:
+//   1 sequence    32 columns 27.7 / 30.1   64: 28.3 / 31.2   128: 38.9 / 32.0
+//   16 sequences  32 columns 69.8 / 106    64: 119 / 107     128: 217 / 106
 bool use_tc(int dtype, int max_rows, int ratio) { return dtype != QMK_FP32 && (long long)max_rows * ratio >= 64; }
 
 int check_attend(const char *who, const QmkKvCache *c, const QmkKvRows *r, int num_q_heads, int dtype) {

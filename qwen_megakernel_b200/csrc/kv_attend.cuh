@@ -53,9 +53,8 @@ __device__ __forceinline__ long long quotient(long long a, long long b) {
   return a / b;
 }
 
-// sum of floor((a i + b) / m) over i < k, by the Euclidean exchange of a and
-// m; the first step by itself, for M is a power of two.  a < 2^9, b < 2^31, k
-// a k + b below 2^31 + 2^25.
+// sum of floor((a i + b) / M) over i < k, by the Euclidean exchange of a and
+// the divisor; the first step by itself, for M is a power of two.
 template <unsigned M>
 __device__ inline long long floor_sum(unsigned k, unsigned a, unsigned b) {
   if (k == 0) return 0;
@@ -64,7 +63,7 @@ __device__ inline long long floor_sum(unsigned k, unsigned a, unsigned b) {
   a %= M;
   b %= M;
   while (a > 0) {
-    const unsigned y = a * k + b;  // (a, b < m <= 2^9, k < 2^17)
+    const unsigned y = a * k + b;  // (a, b < M <= 2^7: below 2^32 for k < 2^24 row blocks)
     if (y < m) break;
     k = y / m;
     b = y % m;
@@ -156,7 +155,7 @@ __device__ inline Range find_range(const Rows &R, int rb, int per_seg, long long
   int at = 0;
   for (int i = lane; i < THREADS; i += 32) at += s_before[i] <= r.u0;
   at = max(0, __reduce_add_sync(0xffffffffu, at) - 1);
-  r.b = at * each;
+  r.b = min(at * each, R.segments - 1);  // (past it only where there are no tiles at all)
   r.seg_at = s_before[at];
   return r;
 }

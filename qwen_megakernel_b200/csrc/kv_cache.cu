@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(kThreads) write_kernel(const __grid_constant__
           float x[8];
           unsigned word[BITS / 4];
           raw[k][i].get(x);
-          const __nv_bfloat16 sb = quantize<BITS, 8>(x, word, a.status);
+          const __nv_bfloat16 sb = quantize<BITS, 8>(x, word, a.status, ok[k]);
           if (ok[k]) {
             const int r = r0 + k * lines + line;
             uint8_t *dst = codes[i] + tab.code[r];

@@ -49,8 +49,8 @@ __device__ __forceinline__ int locate_row(const Rows &R, int r, int &seq, int &p
     b = lo;
     i = r - max(R.row_offsets[b], 0);
     if (i < 0 || r >= R.row_offsets[b + 1]) return 0;
-    if (i >= R.max_rows) return -1;
   }
+  if (i >= R.max_rows) return -1;
   seq = segment_seq(R, b);
   const int start = R.start[b];
   if (seq < 0 || seq >= R.num_seqs || start < 0 || start >= R.max_seq_len || i >= R.max_seq_len - start) return -1;
@@ -141,10 +141,11 @@ __device__ __forceinline__ void codes_any(const float (&x)[N], float s, unsigned
 }
 
 // Codes (packed from the low bits) and scale of a thread's N values; the 32 / N
-// neighbouring lanes of a group agree.  All lanes of the warp call it.
+// neighbouring lanes of a group agree.  All lanes of the warp call it; what a
+// lane without values (!live) gets means nothing.
 template <int BITS, int N>
 __device__ __forceinline__ __nv_bfloat16 quantize(const float (&x)[N], unsigned (&word)[(N * BITS + 31) / 32],
-                                                  unsigned *status) {
+                                                  unsigned *status, bool live = true) {
   constexpr float kTop = BITS == 4 ? 7.f : 127.f;
   unsigned top = 0;  // bits of the largest magnitude, infinities and NaN above all
 #pragma unroll
@@ -152,7 +153,7 @@ __device__ __forceinline__ __nv_bfloat16 quantize(const float (&x)[N], unsigned 
 #pragma unroll
   for (int o = 1; o < kGroup / N; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
   // largest magnitude within 2^-90 .. 2^126: scale and quotients are ordinary numbers
-  const bool easy = top >= 0x12800000u && top < 0x7e800000u;
+  const bool easy = !live || (top >= 0x12800000u && top < 0x7e800000u);
   if (__all_sync(0xffffffffu, easy)) {
     const __nv_bfloat16 sb = __float2bfloat16_rn(divide(__uint_as_float(top), kTop, 1.f / kTop));
     const float s = __bfloat162float(sb), r = fast_rcp(s);
@@ -181,7 +182,7 @@ __device__ __forceinline__ __nv_bfloat16 quantize(const float (&x)[N], unsigned 
   }
 #pragma unroll
   for (int o = 1; o < kGroup / N; o <<= 1) fin = max(fin, __shfl_xor_sync(0xffffffffu, fin, o));
-  if (top >= 0x7f800000u && status) atomicOr(status, QMK_KV_NONFINITE);
+  if (live && top >= 0x7f800000u && status) atomicOr(status, QMK_KV_NONFINITE);
   const __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(__uint_as_float(fin), kTop));
   codes_any<BITS, N>(x, __bfloat162float(sb), word);
   return sb;

@@ -213,7 +213,7 @@ def test_attend_single_rows(dtype, bits, d, hk, ratio):
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("bits", [4, 8])
-@pytest.mark.parametrize("d,hk,ratio", [(128, 2, 2), (64, 1, 8), (128, 1, 1), (64, 2, 3)])
+@pytest.mark.parametrize("d,hk,ratio", [(128, 2, 2), (64, 1, 8), (128, 1, 1), (64, 2, 3), (128, 1, 7), (64, 1, 16)])
 @pytest.mark.parametrize("counts", [(2, 1, 3), (5, 0, 9), (33, 17, 1), (64, 65, 63), (1, 200, 0), (257, 130, 2)], ids=str)
 def test_attend_segments(dtype, bits, d, hk, ratio, counts):
     """Segments of several rows: chunks at positions off the tile borders, a
@@ -343,6 +343,32 @@ def test_wild_offsets_stay_inside():
         torch.cuda.synchronize()
         assert (wide[:8] == 5.0).all() and (wide[16:] == 5.0).all()
         f.cache.status.zero_()
+
+
+@pytest.mark.parametrize("rows", [1, 100])
+def test_segments_without_rows(rows):
+    """Device offsets that give no segment a row: nothing is read or written."""
+    f = Filled([50, 50], hk=1, d=64, seed=1)
+    dev = dict(dtype=torch.int32, device="cuda")
+    r = KVRows.from_tensors(torch.tensor([10, 20], **dev), torch.zeros(3, **dev), rows=100, max_rows=min(rows, 50))
+    q = torch.randn(100, 2, 64, device="cuda", dtype=torch.bfloat16)
+    out = torch.full_like(q, 5.0)
+    f.cache.attend(q, r, out=out)
+    assert (out == 5.0).all() and not f.cache.attend(q, r).any()
+    before = f.cache.k_codes.clone()
+    f.cache.write(out[:, :1], out[:, :1], r)
+    assert torch.equal(f.cache.k_codes, before) and not f.cache.read(r)[0].any()
+    f.cache.check_status()
+
+
+@pytest.mark.parametrize("rows", [1, 3, 90])
+def test_attend_in_place(rows):
+    """out may be q itself."""
+    f = Filled([600], hk=2, d=128, seed=21)
+    q = torch.randn(rows, 4, 128, generator=f.gen, device="cuda", dtype=torch.bfloat16)
+    r = KVRows([600 - rows], [rows])
+    want = f.cache.attend(q, r)
+    assert torch.equal(f.cache.attend(q, r, out=q), want)
 
 
 def test_offsets_past_32_bits():
