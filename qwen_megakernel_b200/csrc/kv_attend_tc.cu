@@ -17,12 +17,17 @@
 // order that decoding leaves them in, in Q, K and V alike, and put back when O
 // is stored.
 //
-// The tensor cores need 4 x 512 cycles for A and B, the 2 x 128 x 128
-// exponentials 2048 on the special-function units, the instructions around
-// them (about 2400 of softmax a line tile, 3200 of decoding for both) as much
-// again: while A's softmax runs, B's products do, and the other way round, and
-// decoding is shared by both.  One line tile of 128 with its own double-
-// buffered S and P took 2.4 times as long a tile: the softmax was waited for.
+// A pair of line tiles needs 4 x 512 cycles of the tensor cores, 2048 of the
+// special-function units for its exponentials and about 11,600 warp
+// instructions (2,900 cycles of four issue ports); while A's softmax runs, B's
+// products do, and the other way round, and decoding is shared by both.  It
+// takes about 5k: what bounds it is the chain of one line tile, scores -> 2.5k
+// cycles of softmax by one warp a scheduler -> P stored -> P V.  Measured, 1023
+// rows at the end of an 8k prompt (4 bits x 128, 16 q and 8 K/V heads): 118 us,
+// 64.4 GFLOP, 546 TFLOP/s, the tensor pipe active 32 % of the time; the same
+// with one line tile of 128 a CTA, S and P double-buffered, 212 us.  A fresh
+// prompt of 1024 tokens takes 50 us, most of it what an item costs whatever its
+// length (plan, queries, output, parts and their merge: about 20 us).
 //
 // Work division, parts and their merge are those of kv_attend.cu, a CTA being
 // one worker.  Warps: 0 TMA, 1 MMA issue, 4-11 softmax and output of A and B,
