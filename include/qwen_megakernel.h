@@ -477,8 +477,8 @@ typedef struct QmkKvTensor {
 #define QMK_KV_TIMEOUT 4u
 #define QMK_KV_COPIES_PENDING 8u
 
-/* Quantize rows of k and v into the cache.  A position that a call writes
- * twice holds either row, value group by value group. */
+/* Quantize rows of k and v into the cache.  A call must not write a position
+ * twice: which codes and which scales stay is then not defined. */
 int qmk_kv_write(const QmkKvCache *cache, const QmkKvRows *rows, const QmkKvTensor *k, const QmkKvTensor *v,
                  unsigned int *status, cudaStream_t stream);
 
@@ -490,8 +490,8 @@ int qmk_kv_read(const QmkKvCache *cache, const QmkKvRows *rows, const QmkKvTenso
  * num_q_heads a multiple (1 .. QMK_KV_MAX_RATIO) of num_kv_heads, q head j
  * reading K/V head j / (num_q_heads / num_kv_heads).  The row at position p
  * attends to positions 0 .. p of its sequence, which must have been written:
- *   out = sum_j softmax_j(scale * q . k_j) v_j.
- * out has q's type.  Scores, sums and the softmax are fp32.  A wait that
+ *   out = sum_j softmax_j(scale * q . k_j) v_j,   scale finite.
+ * out has q's type, and may be q itself.  Scores, sums and the softmax are fp32.  A wait that
  * exceeds 1 s sets QMK_KV_TIMEOUT (the outputs are then invalid), and
  * QMK_KV_COPIES_PENDING if copies were still in flight a second later.
  * The workspace (qmk_kv_attend_workspace_bytes, 256-byte aligned) needs no

@@ -24,6 +24,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <cmath>
 #include <mutex>
 
 #include "kv_attend.cuh"
@@ -809,6 +810,7 @@ extern "C" int qmk_kv_attend(const QmkKvCache *cache, const QmkKvRows *rows, con
   if (rc == QMK_OK) rc = check_tensor(who, "out", out);
   if (rc != QMK_OK) return rc;
   if (q->dtype != out->dtype) return fail(QMK_ERR_ARGS, "%s: out has another type than q", who);
+  if (!(fabsf(scale) < INFINITY)) return fail(QMK_ERR_ARGS, "%s: scale is not finite", who);
   const size_t need = workspace_need(cache, rows, num_q_heads, q->dtype);
   if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256)
     return fail(QMK_ERR_WORKSPACE, "%s: workspace needs %zu bytes, 256-byte aligned", who, need);

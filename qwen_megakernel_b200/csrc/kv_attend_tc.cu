@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
           }
           uint8_t *dst = smem + S::kRaw + st * S::kRawSlot;
           mbar_arrive_expect_tx(&B.raw_full[st], S::kRawBytes);
-          tma_load_4d(dst, side ? &a.v_map : &a.k_map, 0, pos * S::kRowBytes / 128, it.h, sg.seq, &B.raw_full[st]);
+          tma_load_4d(dst, side ? &a.v_map : &a.k_map, 0, pos / (128 / S::kRowBytes), it.h, sg.seq, &B.raw_full[st]);
           bulk_g2s(dst + S::kCodeBytes, (side ? a.v_scales : a.k_scales) + sc + (size_t)pos * G, S::kScaleBytes,
                    &B.raw_full[st], pol);
           ++sent;

@@ -8,10 +8,12 @@
 // of 32, so the group's largest magnitude is two shuffles.  A CTA looks its
 // rows' sequences and positions up once, in shared memory.
 //
-// Measured, 32,368 rows of 8 x 128 bf16, 4 bits: written in 57 us (170 MB, 3.0
-// TB/s; 15 warp instructions a value pair, the loads' latency the rest), read
-// back in 35 us (170 MB, 4.8 TB/s).  With the row looked up by every thread and
-// a correctly rounded division a value it was 127 us.
+// Measured, 32,368 rows of 8 x 128 bf16, 4 bits: written and read back in 86 us,
+// 51 and 35 us (170 MB each, 3.3 and 4.8 TB/s).  The write runs 15 instructions
+// a value (the exact quotient 4 of them) at half the issue rate, the loads'
+// latency the rest: 4 CTAs an SM of 64 registers 86 us, 3 of 70 92, one row a
+// thread in flight 95, four 102.  With the row looked up by every thread and a
+// correctly rounded division a value the pair took 161 us.
 
 #include <algorithm>
 #include <cstdarg>
@@ -155,7 +157,7 @@ struct Raw {
 };
 
 template <typename T, int BITS, int D, bool VEC>
-__global__ void __launch_bounds__(kThreads) write_kernel(const __grid_constant__ Args<T> a) {
+__global__ void __launch_bounds__(kThreads, 4) write_kernel(const __grid_constant__ Args<T> a) {
   __shared__ RowTable tab;
   qmk::pdl_wait();  // rows and cache may be touched by the previous kernel
   qmk::pdl_trigger();

@@ -97,8 +97,8 @@ class KVRows:
         [segments] or None (segment b is sequence b).  With ``row_offsets``,
         ``rows`` is the number of rows of the call's tensors and ``max_rows``
         the most that a segment may hold.  Nothing of the tensors is known on
-        the host: a row out of range is reported by ``check_status``, and a
-        position written twice in one call holds either row."""
+        the host: a row out of range is reported by ``check_status``; a write
+        must not hold a position twice (what stays is then not defined)."""
         self = cls.__new__(cls)
         if row_offsets is None:
             if rows not in (None, start.numel()) or max_rows not in (None, 1):

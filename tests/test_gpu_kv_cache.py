@@ -61,7 +61,7 @@ def check_attend(got, q, k, v, limits, bits, scale):
     """got against the formulas."""
     ref, A = attention(q, k, v, limits, scale)
     seen = k[:max(limits)].abs().repeat_interleave(q.shape[1] // k.shape[1], 1)
-    K = scale * torch.einsum("nhd,mhd->nhm", q.double().abs(), seen).amax(-1, keepdim=True)
+    K = abs(scale) * torch.einsum("nhd,mhd->nhm", q.double().abs(), seen).amax(-1, keepdim=True)
     low = q.dtype != torch.float32
     P = 3 * 2.0**-11 if low else 2.0**-20
     if low and bits == 8:
@@ -241,6 +241,7 @@ def test_attend_peaked_and_spread_scores(dtype, rows):
         f.check(f.cache.attend(q, KVRows([400 - rows], [rows])), q, segs)
     q = g.to(dtype)
     f.check(f.cache.attend(q, KVRows([400 - rows], [rows]), scale=0.5), q, segs, scale=0.5)
+    f.check(f.cache.attend(q, KVRows([400 - rows], [rows]), scale=-0.2), q, segs, scale=-0.2)
     q = torch.zeros_like(q)
     f.check(f.cache.attend(q, KVRows([400 - rows], [rows])), q, segs)
 

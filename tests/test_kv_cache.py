@@ -112,6 +112,8 @@ def test_c_entries_refuse_mixed_types_heads_and_workspaces(lib):
         assert lib.qmk_kv_attend(c, r, t, heads, t, 1.0, FAKE, 1 << 30, None, None) == QMK_ERR_ARGS
         assert lib.qmk_kv_attend_workspace_bytes(c, r, heads, 0) == 0
     assert lib.qmk_kv_attend_workspace_bytes(c, r, 16, 7) == 0
+    for scale in (float("nan"), float("inf"), -float("inf")):
+        assert lib.qmk_kv_attend(c, r, t, 16, t, scale, FAKE, 1 << 30, None, None) == QMK_ERR_ARGS
     need = lib.qmk_kv_attend_workspace_bytes(c, r, 16, 0)
     assert need > 0 and need % 256 == 0
     for ws, n in ((None, need), (FAKE, need - 1), (FAKE + 128, need)):
