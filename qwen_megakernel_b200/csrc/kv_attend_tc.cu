@@ -78,7 +78,9 @@ struct TcBars {
   uint64_t raw_full[4], raw_empty[4];
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];  // decoded tiles; empty: read by the MMAs
   uint64_t s_full[2], p_full[2], pv[2];             // of A and B; pv: P V of a tile done
-  uint64_t q_full, drain;
+  // queries in place, of A and B apart: where B has no lines its warps wait for
+  // nothing and may be items ahead, so an arrival of theirs must not count for A
+  uint64_t q_full[2], drain;
   float exp_k[4], exp_v[4];  // 2^E of K and E of V, of tile t in slot t % 4
   uint32_t tmem;
   int abort;
@@ -271,8 +273,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
       mbar_init(&B.s_full[i], 2);  // the MMAs' commit, and the issuer itself: it passes the exponents on
       mbar_init(&B.p_full[i], 4);
       mbar_init(&B.pv[i], 1);
+      mbar_init(&B.q_full[i], 4);
     }
-    mbar_init(&B.q_full, 8);
     mbar_init(&B.drain, 1);
     fence_mbar_init();
     B.abort = 0;
@@ -372,11 +374,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
       tc_fence_after_sync();
       return true;
     };
-    unsigned item = 0;
+    unsigned n_q[2] = {0, 0};
     items([&](const Item &it, int nt) {
       if (nt == 0) return true;
       const bool two = it.nrows * hb > kHalf;
-      if (!wait_warp(&B.q_full, item++ & 1, abort)) return false;
+      if (!wait_warp(&B.q_full[0], n_q[0]++ & 1, abort)) return false;
+      if (two && !wait_warp(&B.q_full[1], n_q[1]++ & 1, abort)) return false;
       if (!tiles_ready(t)) return false;
       scores(0, t, !two);
       if (two) scores(1, t, true);
@@ -455,7 +458,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) attend_tc_kernel(const __grid_c
         fence_proxy_async_smem();
       }
       __syncwarp();
-      if (nt > 0 && lane == 0) mbar_arrive(&B.q_full);
+      if (nt > 0 && !idle && lane == 0) mbar_arrive(&B.q_full[x]);
       float R = -INFINITY, l = 0.f;
       for (int i = 0; i < (idle ? 0 : nt); ++i, ++n_s) {
         const unsigned g = t + i;

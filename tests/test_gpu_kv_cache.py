@@ -230,6 +230,29 @@ def test_attend_segments(dtype, bits, d, hk, ratio, counts):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("hk,ratio", [(8, 2), (4, 13), (2, 16)], ids=str)
+def test_single_rows_among_prompts(hk, ratio, dtype):
+    """Blocks of few rows one after another and between full ones: whatever
+    order a worker meets them in, no row takes another's query."""
+    lens = [5, 60, 128, 129, 300, 957, 700]
+    f = Filled(lens, hk=hk, seed=ratio)
+    segs = []
+    for i in range(60):
+        s = i % 5
+        segs.append((s, (37 * i) % lens[s], 1))
+        if i % 20 == 7:
+            segs.append((5, 15 * i, 249 if ratio == 13 else 130))
+        if i % 20 == 15:
+            segs.append((6, 3 * i, 33))
+    q = torch.randn(sum(n for _, _, n in segs), hk * ratio, 128, generator=f.gen, device="cuda").to(dtype)
+    rows = KVRows([a for _, a, _ in segs], [n for _, _, n in segs], [s for s, _, _ in segs])
+    for _ in range(3):
+        got = f.cache.attend(q, rows)
+        f.cache.check_status()
+        f.check(got, q, segs)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("rows", [1, 40, 150])
 def test_attend_peaked_and_spread_scores(dtype, rows):
     """Scores up to several hundred (one position takes all) and all alike."""
